@@ -34,6 +34,10 @@
  *                             split across devices (the reference has no context parallelism)
  *   rp_fp8_gemm_qkv_quant  <- the QKV projection followed by the eager quantize of Q, K, V,
  *                             fp8_flash_attn_hopper.py:474-480 (per-128-token-block mode)
+ *   rp_paged_append, rp_paged_decode, rp_paged_evict <- (no reference kernel: its token-VLA decode
+ *                             keeps its cache in HF generate, scripts/run_vla_openvla_gpu.py:174-186)
+ *   rp_token_logprobs      <- (no reference kernel: scores of the sampled candidates of
+ *                             VLAEngine.plan, models/vla.py:229-258)
  */
 #ifndef REPERCEP_B200_H_
 #define REPERCEP_B200_H_
@@ -45,7 +49,7 @@
 extern "C" {
 #endif
 
-#define RP_ABI_VERSION 4
+#define RP_ABI_VERSION 5
 
 typedef enum rp_status {
   RP_OK = 0,
@@ -69,7 +73,8 @@ typedef enum rp_p_mode {
 
 typedef enum rp_dtype {
   RP_DTYPE_BF16 = 0,
-  RP_DTYPE_F16 = 1
+  RP_DTYPE_F16 = 1,
+  RP_DTYPE_F32 = 2 /* logits only */
 } rp_dtype;
 
 /* ABI version compiled into the library (RP_ABI_VERSION). */
@@ -286,6 +291,112 @@ int rp_fp8_gemm_qkv_quant(const void* a, int64_t lda, const void* w, int64_t ldw
  * for the A operand, per-output-channel weight scales for an RP_B_NK B. */
 int rp_quant_fp8_rows(const void* x, int64_t ldx, int in_dtype, int rows, int cols, void* out,
                       int64_t ldo, float* scales, void* stream);
+
+/* ------------------------------------------- paged key-value cache
+ * A pool of pages of page_size token slots each.  Position p of sequence b is
+ * slot p % page_size of page page_table[b * table_stride + p / page_size];
+ * tables and lengths are int32 on the device.  Sequences may share pages.
+ *   k, v       row (page, head, slot) at base + (page * strides[0] + head *
+ *              strides[1] + slot * strides[2]) elements, head_dim elements
+ *              of dtype (one set of strides for both; 16-byte multiples)
+ *   k_scales, v_scales   RP_KV_E4M3 only: fp32 dequant multipliers of the
+ *              rows, contiguous (num_pages, heads, page_size)
+ * head_dim in {32, 64, 128, 256}; any page_size.
+ * What only the device can see is checked there: a page id outside the pool
+ * (0x201), a length below 0 or past the page table (0x202) and a token id
+ * past the vocabulary (0x203) are recorded in the device status word and
+ * never read or written through: such a row is skipped, such a length is cut
+ * to the nearest valid one. */
+typedef enum rp_kv_dtype {
+  RP_KV_BF16 = 0,
+  RP_KV_F16 = 1,
+  RP_KV_E4M3 = 2 /* one scale per row: rp_quant_fp8_rows's recipe on a row of K or V */
+} rp_kv_dtype;
+
+typedef struct rp_paged_kv {
+  void* k;
+  void* v;
+  float* k_scales;
+  float* v_scales;
+  int64_t strides[3]; /* elements: page, head, slot */
+  int dtype;          /* rp_kv_dtype */
+  int num_pages, heads, page_size, head_dim;
+} rp_paged_kv;
+
+/* New tokens' K and V rows into the cache, quantized when it is e4m3.
+ *   k_new, v_new  bf16 or fp16 (in_dtype; a 16-bit cache's own type), row
+ *                 (token, head) at token * new_strides[0] + head *
+ *                 new_strides[1] (k), [2], [3] (v); multiples of 8 elements
+ *   starts        (B + 1) int32 first new token of each sequence: token t of
+ *                 starts[b] <= t < starts[b + 1] goes to position lengths[b]
+ *                 + t - starts[b]; tokens outside [starts[0], starts[B]) are
+ *                 left out.  NULL: token b is sequence b's one new token
+ *   weights       NULL or accumulated attention weights (B, heads,
+ *                 weight_cols) at b * weight_strides[0] + h *
+ *                 weight_strides[1] + p: zeroed at the new positions
+ *   lengths_out   (B) lengths after the call; not the memory of lengths */
+int rp_paged_append(const rp_paged_kv* kv, const void* k_new, const void* v_new,
+                    const int64_t* new_strides, int in_dtype, int tokens, const int32_t* starts,
+                    const int32_t* page_table, int64_t table_stride, int table_pages,
+                    const int32_t* lengths, int B, float* weights, const int64_t* weight_strides,
+                    int64_t weight_cols, int32_t* lengths_out, void* stream);
+
+/* Workspace bytes rp_paged_decode needs. */
+int rp_paged_decode_workspace_bytes(const rp_paged_kv* kv, int B, int Hq, int table_pages,
+                                    int with_weights, size_t* bytes);
+
+/* Attention of one new token per sequence over its lengths[b] cached tokens.
+ *   q    (B, Hq, head_dim) bf16 or fp16 (q_dtype; a 16-bit cache's own type)
+ *        at b * q_strides[0] + h * q_strides[1]; query head h reads KV head
+ *        h / (Hq / heads)
+ *   out  (B, Hq, head_dim) in q's type, element strides out_strides[2]
+ *   lse  NULL or (B, Hq) fp32, the natural log of each row's sum of exps
+ *   weights  NULL or (B, heads, weight_cols) as in rp_paged_append: every
+ *        key's attention weight, summed over the query heads of its KV head,
+ *        is added.  No atomics: the sums do not depend on the order of
+ *        execution
+ * A sequence of length 0 gives out = 0 and lse = -inf.  sm_scale <= 0 selects
+ * 1/sqrt(head_dim).  Scores, sums and accumulators are fp32; softmax weights
+ * are rounded to 16 bits for their product with V (fp16 unless the cache is
+ * bf16). */
+int rp_paged_decode(const rp_paged_kv* kv, const void* q, const int64_t* q_strides, int q_dtype,
+                    int B, int Hq, const int32_t* page_table, int64_t table_stride,
+                    int table_pages, const int32_t* lengths, float sm_scale, void* out,
+                    const int64_t* out_strides, float* lse, float* weights,
+                    const int64_t* weight_strides, int64_t weight_cols, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
+/* Cuts every sequence to at most `budget` tokens per KV head: a sequence of n
+ * > budget tokens keeps its last `recent` ones and, of the older, the budget -
+ * recent of greatest accumulated weight (ties: the lowest position; NaN above
+ * everything).  Kept rows move, in order, to positions 0, 1, ... of out_table's
+ * pages in the same pool; a shorter sequence moves whole.  Nothing is written
+ * to page_table's pages (other sequences may share them), so out_table's must
+ * be other ones.
+ *   kept         (B, heads, budget) int32 old positions, -1 past the end
+ *   lengths_out  (B) int32 min(n, budget)
+ *   weights_out  (B, heads, out_pages * page_size) fp32 the kept tokens'
+ *                weights, 0 past the end */
+int rp_paged_evict(const rp_paged_kv* kv, const int32_t* page_table, int64_t table_stride,
+                   int table_pages, const int32_t* lengths, int B, const float* weights,
+                   const int64_t* weight_strides, int64_t weight_cols, const int32_t* out_table,
+                   int64_t out_stride, int out_pages, int budget, int recent, int32_t* kept,
+                   int32_t* lengths_out, float* weights_out, void* stream);
+
+/* Scores of sampled tokens from logits (rows, vocab) bf16, fp16 or fp32
+ * (dtype), row r at logits + r * row_stride elements (any alignment to the
+ * type):
+ *   logprobs      (rows) log probability of tokens[r]; 0 for a negative token
+ *                 (none), NaN for one past the vocabulary
+ *   entropy       (rows) -sum p log p
+ *   top_logprobs, top_ids  (rows, top) the `top` (0..64) largest log
+ *                 probabilities and their token ids, ties to the lowest id
+ * All sums are fp32.  -inf logits have probability 0; a row of nothing else
+ * has entropy 0 and log probabilities -inf; NaN or +inf in a row makes its
+ * sums NaN (NaN counts as the largest value among the alternatives). */
+int rp_token_logprobs(const void* logits, int64_t row_stride, int dtype, int rows, int vocab,
+                      const int64_t* tokens, int top, float* logprobs, float* entropy,
+                      float* top_logprobs, int64_t* top_ids, void* stream);
 
 #ifdef __cplusplus
 }

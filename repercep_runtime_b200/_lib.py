@@ -21,6 +21,10 @@ RP_P_E4M3 = 0
 RP_P_E4M3_HILO = 1
 RP_DTYPE_BF16 = 0
 RP_DTYPE_F16 = 1
+RP_DTYPE_F32 = 2
+RP_KV_BF16 = 0
+RP_KV_F16 = 1
+RP_KV_E4M3 = 2
 RP_B_KN = 0
 RP_B_NK = 1
 RP_QUANT_PHASE_AMAX = 1
@@ -40,6 +44,28 @@ _c_int = ctypes.c_int
 _c_float = ctypes.c_float
 _c_size_t = ctypes.c_size_t
 _c_i64_p = ctypes.POINTER(ctypes.c_int64)
+
+_c_i64 = ctypes.c_int64
+
+
+class PagedKVStruct(ctypes.Structure):
+    """``rp_paged_kv`` of include/repercep_b200.h."""
+
+    _fields_ = [
+        ("k", _c_void_p),
+        ("v", _c_void_p),
+        ("k_scales", _c_void_p),
+        ("v_scales", _c_void_p),
+        ("strides", _c_i64 * 3),
+        ("dtype", _c_int),
+        ("num_pages", _c_int),
+        ("heads", _c_int),
+        ("page_size", _c_int),
+        ("head_dim", _c_int),
+    ]
+
+
+_c_kv_p = ctypes.POINTER(PagedKVStruct)
 
 # name -> (restype, argtypes); mirrors include/repercep_b200.h
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
@@ -208,9 +234,35 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
             _c_void_p,
         ],
     ),
+    "rp_paged_append": (
+        _c_int,
+        [_c_kv_p, _c_void_p, _c_void_p, _c_i64_p, _c_int, _c_int, _c_void_p]
+        + [_c_void_p, _c_i64, _c_int, _c_void_p, _c_int]
+        + [_c_void_p, _c_i64_p, _c_i64, _c_void_p, _c_void_p],
+    ),
+    "rp_paged_decode_workspace_bytes": (
+        _c_int,
+        [_c_kv_p, _c_int, _c_int, _c_int, _c_int, ctypes.POINTER(_c_size_t)],
+    ),
+    "rp_paged_decode": (
+        _c_int,
+        [_c_kv_p, _c_void_p, _c_i64_p, _c_int, _c_int, _c_int]
+        + [_c_void_p, _c_i64, _c_int, _c_void_p, _c_float, _c_void_p, _c_i64_p, _c_void_p]
+        + [_c_void_p, _c_i64_p, _c_i64, _c_void_p, _c_size_t, _c_void_p],
+    ),
+    "rp_paged_evict": (
+        _c_int,
+        [_c_kv_p, _c_void_p, _c_i64, _c_int, _c_void_p, _c_int]
+        + [_c_void_p, _c_i64_p, _c_i64, _c_void_p, _c_i64, _c_int, _c_int, _c_int]
+        + [_c_void_p, _c_void_p, _c_void_p, _c_void_p],
+    ),
+    "rp_token_logprobs": (
+        _c_int,
+        [_c_void_p, _c_i64, _c_int, _c_int, _c_int, _c_void_p, _c_int] + [_c_void_p] * 5,
+    ),
 }
 
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None

@@ -161,6 +161,7 @@ int set_last_error(int code, const char* fmt, ...) {
   g_last_error = buf;
   return code;
 }
+int device_ready(int** status) { return ::device_ready(status); }
 }  // namespace rp
 
 namespace {

@@ -10,6 +10,9 @@ namespace rp {
 
 // Records `fmt` as the calling thread's rp_last_error() message; returns code.
 int set_last_error(int code, const char* fmt, ...);
+// RP_OK and the device status word when the current device is sm_100, else
+// an rp_status (with its message recorded).
+int device_ready(int** status);
 
 // ------------------------------------------------------------- quantize
 constexpr int kQuantRows = 128;     // tokens per scale block / per CTA
