@@ -6,129 +6,885 @@
 //   out_g = sum_j 2^(s_gj - m_g) v_j / l_g,  lse_g = ln 2 * (m_g + log2 l_g)
 // (s in log2 units), and on request w[b, h, j] += sum_g 2^(s_gj - m_g) / l_g.
 // A sequence without tokens gives out = 0 and lse = -inf.
+//
+// Every cached row is read once and meets G queries only, so the kernel is
+// bound by HBM: its work is to keep enough bytes in flight on every SM.
+//  - Work: the tiles (64 or 128 keys) of all (sequence, KV head) items in one
+//    line, cut into equal runs, one per resident CTA, whatever the lengths.  An
+//    item inside one run is finished there; an item that a cut splits leaves
+//    (m, l, O) partials, at most two per CTA, that a second kernel joins in
+//    order.  Workspace and launches do not depend on the lengths, and nothing
+//    is atomic: equal inputs give equal bits.
+//  - Loads: each warp streams its own slice of every tile through a ring of
+//    its own in shared memory (16-byte cp.async, the page ids one step ahead),
+//    so there is no CTA-wide barrier between tiles.
+//  - Products: keys are the 16 rows of mma.m16n8k16 and the group's queries
+//    its 8 columns (S^T = K Q^T, O^T = V^T P^T): a group of up to 8 heads costs
+//    one column block.  At the memory's rate the products take about a tenth
+//    of the tensor pipe's time, which tcgen05's 128-row tiles would not change.
+//  - e4m3 rows are widened to fp16 exactly.  The queries are brought to fp16
+//    by a power of two of their row's maximum, the rows' K scales multiply the
+//    scores in fp32, and their V scales the softmax weights, over a running
+//    power of two that keeps those within fp16's range.
+//  - Rounding: scores, sums and accumulators are fp32; softmax weights are
+//    rounded to the 16-bit operand type for the product with V (relative 2^-8
+//    or 2^-11 of each term, the size of the output's own rounding).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <atomic>
+
 #include "internal.h"
 #include "paged.h"
+#include "ptx.cuh"
 
 namespace rp {
 namespace {
 
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr int kSplits = 16;
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kJoinThreads = 512;
+constexpr int kMaxCtas = 592;  // CTAs of the main kernel, at most
+constexpr int kMinTiles = 2;    // tiles of a CTA's run, at least (but for the last)
+// The running maximum of a row is raised only when a score exceeds it by this
+// much (log2 units): until then 2^(s - m) <= 256, and nothing is rescaled.
+constexpr float kRescale = 8.f;
 
-__device__ __forceinline__ float value16(uint16_t u, bool f16) {
-  return f16 ? __half2float(__ushort_as_half(u)) : __uint_as_float(static_cast<uint32_t>(u) << 16);
+template <int KV, int D, int NT>
+struct Cfg {
+  static constexpr bool kFp8 = KV == kKvE4m3;
+  static constexpr bool kBf16 = KV == kKvBf16;
+  static constexpr int kRow = D * (kFp8 ? 1 : 2);   // bytes of a row
+  static constexpr int kChunks = kRow / 16;         // 16-byte chunks of a row
+  static constexpr int kKeys = kRow >= 256 ? 16 : 32;  // keys of a warp's step
+  static constexpr int kTile = kKeys * kWarps;
+  static constexpr int kRowsBytes = kKeys * kRow;
+  static constexpr int kStage = 2 * kRowsBytes + (kFp8 ? kKeys * 8 : 0);
+  // about 24 KB in flight a warp, two CTAs an SM
+  static constexpr int kStages = 2 * kRowsBytes >= 8192 ? 3 : 2 * kRowsBytes >= 4096 ? 6 : 8;
+  static constexpr int kFrags = D / 16 * NT;  // accumulator fragments (float4 a lane)
+  static constexpr int kRing = kStages * kStage;
+  static constexpr int kSmem = kWarps * kRing + 2 * kFrags * 512 + kWarps * NT * 8 * 8 + kWarps * kStages * 4;
+};
+
+// What a CTA left for the join: the item it began (tile 0) without ending it
+// and the slot of that partial, and the item it continued (slot 0).
+struct Cut {
+  int begun, begun_slot, continued, pad;
+};
+
+struct Params {
+  PagedDecodeArgs a;
+  int G;       // query heads of a KV head
+  int groups;  // column groups of a KV head (NT * 8 query heads each)
+  int shift;   // log2 of the page size, or -1
+  int grid;    // CTAs of the main kernel
+  int score_pitch;
+  float4* part_o;  // (grid * 2, kFrags, 32)
+  float* part_ml;  // (grid * 2, 2, NT * 8)
+  Cut* cuts;       // (grid)
+  float* lse2;     // (B, Hq) log2-sum-exp, with weights only
+  float* scores;   // (B, Hq, score_pitch) log2 units, with weights only
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool read) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(read ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool read) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(read ? 4 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+// 8x8 transpose across the warp: (row lane / 4, columns 2 (lane % 4), + 1).
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (BF16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Two e4m3 values (low 16 bits) as two fp16, exactly.
+__device__ __forceinline__ uint32_t widen_lo(uint32_t x) {
+  uint32_t y;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t widen_hi(uint32_t x) {
+  uint32_t y;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(y) : "r"(x));
+  return y;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  uint32_t y;
+  if constexpr (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+  return y;
+}
+__device__ __forceinline__ float value16(uint32_t u, bool f16) {
+  return f16 ? __half2float(__ushort_as_half(static_cast<uint16_t>(u))) : __uint_as_float(u << 16);
 }
 __device__ __forceinline__ uint16_t round16(float x, bool f16) {
   return f16 ? __half_as_ushort(__float2half_rn(x)) : __bfloat16_as_ushort(__float2bfloat16_rn(x));
 }
-__device__ __forceinline__ float value_kv(const uint8_t* base, int64_t i, int dtype) {
-  if (dtype == kKvE4m3)
-    return __half2float(__half(__nv_cvt_fp8_to_halfraw(base[i], __NV_E4M3)));
-  return value16(reinterpret_cast<const uint16_t*>(base)[i], dtype == kKvF16);
-}
+__device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
 
-// One warp per (sequence, query head, split): keys one after another, each
-// lane D / 32 dimensions.
-template <int D>
-__global__ void decode_kernel(const PagedDecodeArgs a, float* part, float* scores, int cap) {
-  constexpr int E = D / 32;
-  const int lane = threadIdx.x, split = blockIdx.x, hq = blockIdx.y, b = blockIdx.z;
-  const int G = a.Hq / a.kv.heads, h = hq / G;
-  const int n = table_length(a.t, a.kv.page_size, b, a.status);
-  const int per = (n + kSplits - 1) / kSplits;
-  const int j0 = split * per, j1 = min(n, j0 + per);
-  float q[E], o[E], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    q[e] = value16(a.q[b * a.q_seq + hq * a.q_head + e * 32 + lane], a.q_f16);
-    o[e] = 0.f;
+// A place in the line of tiles: sequence, item of the sequence (KV head and
+// column group), tile of the item.
+struct Place {
+  int b, item, tile, n, tiles;
+  template <typename C>
+  __device__ __forceinline__ void enter(const Params& p) {
+    n = table_length(p.a.t, p.a.kv.page_size, b, p.a.status);
+    tiles = (n + C::kTile - 1) / C::kTile;
   }
-  const int32_t* row = a.t.table + b * a.t.stride;
-  for (int j = j0; j < j1; ++j) {
-    const int64_t off = row_offset(a.kv, row, j, h, a.status);
-    float x = -INFINITY, vs = 1.f;
-    if (off >= 0) {
-      x = 0.f;
-#pragma unroll
-      for (int e = 0; e < E; ++e) x += q[e] * value_kv(a.kv.k, off + e * 32 + lane, a.kv.dtype);
-#pragma unroll
-      for (int s = 16; s > 0; s /= 2) x += __shfl_xor_sync(0xffffffffu, x, s);
-      x *= a.scale_log2;
-      if (a.kv.dtype == kKvE4m3) {
-        const int64_t i = scale_index(a.kv, row, j, h);
-        x *= a.kv.ks[i];
-        vs = a.kv.vs[i];
-      }
+  // The next tile; the line goes on (a sequence without tiles has none of it).
+  template <typename C>
+  __device__ __forceinline__ void next(const Params& p) {
+    if (++tile < tiles) return;
+    tile = 0;
+    if (++item < p.a.kv.heads * p.groups) return;
+    item = 0;
+    tiles = 0;
+    while (++b < p.a.t.B && tiles == 0) {
+      enter<C>(p);
+      if (tiles > 0) return;
     }
-    if (scores && lane == 0) scores[(static_cast<int64_t>(b) * a.Hq + hq) * cap + j] = x;
-    const float m1 = (x > m) ? x : m;
-    const float ref = m1 == -INFINITY ? 0.f : m1;
-    const float keep = exp2f(m - ref), p = exp2f(x - ref);
-    m = m1;
-    l = l * keep + p;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      o[e] *= keep;
-      if (off >= 0) o[e] += p * vs * value_kv(a.kv.v, off + e * 32 + lane, a.kv.dtype);
-    }
-  }
-  float* out = part + ((static_cast<int64_t>(b) * a.Hq + hq) * kSplits + split) * (D + 2);
-  if (lane == 0) {
-    out[0] = m;
-    out[1] = l;
-  }
-#pragma unroll
-  for (int e = 0; e < E; ++e) out[2 + e * 32 + lane] = o[e];
-}
-
-// The splits of one (sequence, query head) joined; one thread per dimension.
-__global__ void decode_join_kernel(const PagedDecodeArgs a, const float* part, float* lse2, int D) {
-  const int hq = blockIdx.x, b = blockIdx.y, d = threadIdx.x;
-  const float* in = part + (static_cast<int64_t>(b) * a.Hq + hq) * kSplits * (D + 2);
-  float m = -INFINITY, l = 0.f, o = 0.f;
-  for (int s = 0; s < kSplits; ++s) m = fmaxf(m, in[s * (D + 2)]);
-  const float ref = m == -INFINITY ? 0.f : m;
-  for (int s = 0; s < kSplits; ++s) {
-    const float f = exp2f(in[s * (D + 2)] - ref);
-    l += in[s * (D + 2) + 1] * f;
-    o += in[s * (D + 2) + 2 + d] * f;
-  }
-  a.out[b * a.o_seq + hq * a.o_head + d] = round16(l == 0.f ? 0.f : o / l, a.q_f16);
-  if (d == 0) {
-    lse2[b * a.Hq + hq] = m + log2f(l);
-    if (a.lse) a.lse[b * a.Hq + hq] = kLn2 * (m + log2f(l));
-  }
-}
-
-// Every key's weights, summed over the query heads of its KV head.
-__global__ void decode_weights_kernel(const PagedDecodeArgs a, const float* scores, const float* lse2,
-                                      int cap) {
-  const int j = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y, b = blockIdx.z;
-  if (j >= table_length(a.t, a.kv.page_size, b, a.status)) return;
-  const int G = a.Hq / a.kv.heads;
-  float w = 0.f;
-  for (int g = 0; g < G; ++g) {
-    const int64_t hq = static_cast<int64_t>(b) * a.Hq + h * G + g;
-    const float x = scores[hq * cap + j], y = lse2[hq];
-    w += y == -INFINITY ? 0.f : exp2f(x - y);
-  }
-  a.weights.w[b * a.weights.s_seq + h * a.weights.s_head + j] += w;
-}
-
-struct Workspace {
-  size_t part, lse2, scores, total;
-  Workspace(const PagedPool& kv, int B, int Hq, int table_pages, bool weights) {
-    const size_t heads = static_cast<size_t>(B) * Hq;
-    part = 0;
-    lse2 = heads * kSplits * (kv.D + 2) * 4;
-    scores = lse2 + heads * 4;
-    total = scores + (weights ? heads * table_pages * kv.page_size * 4 : 0);
   }
 };
+
+// Writes one head's output row elements and its log-sum-exp; (m, l) in log2
+// units.
+__device__ __forceinline__ void write_lse(const Params& p, int b, int hq, float m, float l) {
+  const float y = l == 0.f ? -INFINITY : m + log2f(l);
+  if (p.lse2) p.lse2[static_cast<int64_t>(b) * p.a.Hq + hq] = y;
+  if (p.a.lse) p.a.lse[static_cast<int64_t>(b) * p.a.Hq + hq] = kLn2 * y;
+}
+
+// Dimension of accumulator row r (lane / 4, + 8 for the second half) of
+// fragment block dt: e4m3's transposed loads interleave even and odd ones.
+template <bool FP8>
+__device__ __forceinline__ int dim_of(int dt, int r, int half) {
+  return FP8 ? dt * 16 + 2 * r + half : dt * 16 + r + 8 * half;
+}
+
+template <int KV, int D, int NT>
+__global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
+  using C = Cfg<KV, D, NT>;
+  constexpr int MT = C::kKeys / 16, KS = D / 16, DT = D / 16, S = C::kStages;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row = lane >> 2, pair = lane & 3;
+  const uint32_t ring = smem_u32(smem) + warp * C::kRing;
+  float4* join = reinterpret_cast<float4*>(smem + kWarps * C::kRing);
+  float* sm_m = reinterpret_cast<float*>(smem + kWarps * C::kRing + 2 * C::kFrags * 512);
+  float* sm_l = sm_m + kWarps * NT * 8;
+  uint32_t* live = reinterpret_cast<uint32_t*>(sm_l + kWarps * NT * 8) + warp * S;
+  const PagedPool& kv = p.a.kv;
+  const int items = kv.heads * p.groups, B = p.a.t.B;
+
+  // ---- this CTA's run of tiles: a prefix sum over the sequences
+  __shared__ long long sums[kWarps];
+  __shared__ Place at;
+  const int per = (B + kThreads - 1) / kThreads;
+  const int b0 = threadIdx.x * per, b1 = min(B, b0 + per);
+  long long mine = 0;
+  for (int b = b0; b < b1; ++b)
+    mine += (table_length(p.a.t, kv.page_size, b, p.a.status) + C::kTile - 1) / C::kTile;
+  long long before = mine;
+#pragma unroll
+  for (int s = 1; s < 32; s *= 2) {
+    const long long x = __shfl_up_sync(0xffffffffu, before, s);
+    if (lane >= s) before += x;
+  }
+  if (lane == 31) sums[warp] = before;
+  __syncthreads();
+  long long total = 0;
+  before -= mine;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += sums[w];
+    total += sums[w];
+  }
+  total *= items;
+  // every run up to `runs` has a tile, so an item's parts lie in CTAs next to each other
+  const long long runs = min(static_cast<long long>(p.grid), (total + kMinTiles - 1) / kMinTiles);
+  const bool idle = blockIdx.x >= runs;
+  const long long first = idle ? 0 : total * blockIdx.x / runs, last = idle ? 0 : total * (blockIdx.x + 1) / runs;
+  if (first < last && before * items <= first && first < (before + mine) * items) {
+    Place x;
+    long long skip = first - before * items;
+    for (x.b = b0;; ++x.b) {
+      x.enter<C>(p);
+      if (skip < static_cast<long long>(x.tiles) * items) break;
+      skip -= static_cast<long long>(x.tiles) * items;
+    }
+    x.item = static_cast<int>(skip / x.tiles);
+    x.tile = static_cast<int>(skip % x.tiles);
+    at = x;
+  }
+  // sequences without tokens: zeros
+  for (int b = blockIdx.x; b < B; b += p.grid) {
+    if (table_length(p.a.t, kv.page_size, b, p.a.status) > 0) continue;
+    for (int i = threadIdx.x; i < p.a.Hq * D; i += kThreads)
+      p.a.out[b * p.a.o_seq + (i / D) * p.a.o_head + i % D] = 0;
+    for (int i = threadIdx.x; i < p.a.Hq; i += kThreads) write_lse(p, b, i, 0.f, 0.f);
+  }
+  __syncthreads();
+  Cut cut{-1, 0, -1, 0};
+  if (first == last) {
+    if (threadIdx.x == 0) p.cuts[blockIdx.x] = cut;
+    return;
+  }
+  Place load = at, here = at;
+  int to_load = static_cast<int>(last - first), left = to_load;
+
+  // ---- loads: lane's key of the warp's slice, its page id one step ahead
+  const int my_key = lane % C::kKeys;
+  int page = 0;
+  const auto fetch_page = [&] {
+    const int key = load.tile * C::kTile + warp * C::kKeys + my_key;
+    page = -1;
+    if (to_load > 0 && key < load.n) {
+      const int i = p.shift >= 0 ? key >> p.shift : key / kv.page_size;
+      page = __ldg(p.a.t.table + load.b * p.a.t.stride + i);
+    }
+  };
+  const auto issue = [&](int stage) {
+    if (to_load > 0) {
+      const int key = load.tile * C::kTile + warp * C::kKeys + my_key;
+      const int head = load.item / p.groups;
+      const uint32_t base = ring + stage * C::kStage;
+      bool ok = key < load.n;
+      if (ok && static_cast<unsigned>(page) >= static_cast<unsigned>(kv.num_pages)) {
+        atomicCAS(p.a.status, 0, kStatusBadPage);
+        ok = false;
+      }
+      const uint32_t mask = __ballot_sync(0xffffffffu, ok);
+      if (lane == 0) live[stage] = mask;
+      int64_t off = 0;
+      if (ok) {
+        const int slot = p.shift >= 0 ? key & (kv.page_size - 1) : key % kv.page_size;
+        off = page * kv.s_page + head * kv.s_head + slot * kv.s_slot;
+        if constexpr (!C::kFp8) off *= 2;
+        if constexpr (C::kFp8) {
+          const int64_t i = (static_cast<int64_t>(page) * kv.heads + head) * kv.page_size + slot;
+          if (lane < C::kKeys) {
+            cp_async4(base + 2 * C::kRowsBytes + lane * 4, kv.ks + i, true);
+            cp_async4(base + 2 * C::kRowsBytes + (C::kKeys + lane) * 4, kv.vs + i, true);
+          }
+        }
+      } else if constexpr (C::kFp8) {
+        if (lane < C::kKeys) {
+          cp_async4(base + 2 * C::kRowsBytes + lane * 4, kv.ks, false);
+          cp_async4(base + 2 * C::kRowsBytes + (C::kKeys + lane) * 4, kv.vs, false);
+        }
+      }
+      if (key - my_key < load.n) {  // some of the slice is in the sequence: the rest of it is zeroed
+#pragma unroll
+        for (int i = 0; i < C::kKeys * C::kChunks / 32; ++i) {
+          const int c = i * 32 + lane, r = c / C::kChunks, col = c % C::kChunks;
+          const int64_t o = __shfl_sync(0xffffffffu, off, r);
+          const bool read = (mask >> r) & 1;
+          constexpr int kRsh = C::kRow >= 128 ? 0 : C::kRow == 64 ? 1 : 2;
+          constexpr int kMask = C::kChunks >= 8 ? 7 : C::kChunks - 1;
+          const uint32_t dst = base + r * C::kRow + ((col ^ ((r >> kRsh) & kMask)) << 4);
+          cp_async16(dst, kv.k + o + col * 16, read);
+          cp_async16(dst + C::kRowsBytes, kv.v + o + col * 16, read);
+        }
+      }
+      --to_load;
+      if (to_load > 0) load.next<C>(p);
+      fetch_page();
+    }
+    cp_commit();
+  };
+  fetch_page();
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) issue(s);
+  int stage = 0;
+
+  bool first_segment = true;
+  while (left > 0) {
+    const int b = here.b, head = here.item / p.groups, g0 = here.item % p.groups * NT * 8;
+    const int cols = min(NT * 8, p.G - g0), hq0 = head * p.G + g0;
+    const int seg = min(left, here.tiles - here.tile);
+    const bool begins = here.tile == 0, ends = here.tile + seg == here.tiles;
+
+    // ---- queries as B operands: column lane / 4, rows 2 (lane % 4) + {0, 1, 8, 9}
+    // (e4m3: 4 (lane % 4) + {0..3}, the order in which its K rows come)
+    uint32_t q[KS][NT][2];
+    float factor[NT][2];  // of the score columns 2 (lane % 4) + {0, 1}
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int col = nt * 8 + row;
+      const uint16_t* src = p.a.q + b * p.a.q_seq + (hq0 + min(col, cols - 1)) * p.a.q_head;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        if constexpr (C::kFp8) {
+          const uint2 w = __ldg(reinterpret_cast<const uint2*>(src + ks * 16 + pair * 4));
+          q[ks][nt][0] = col < cols ? w.x : 0;
+          q[ks][nt][1] = col < cols ? w.y : 0;
+        } else {
+          const uint32_t x = __ldg(reinterpret_cast<const uint32_t*>(src + ks * 16 + pair * 2));
+          const uint32_t y = __ldg(reinterpret_cast<const uint32_t*>(src + ks * 16 + pair * 2 + 8));
+          q[ks][nt][0] = col < cols ? x : 0;
+          q[ks][nt][1] = col < cols ? y : 0;
+        }
+      }
+      if constexpr (C::kFp8) {
+        // fp16 queries: times the power of two that brings the row's maximum to [2^13, 2^14)
+        float top = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            top = fmaxf(top, fmaxf(fabsf(value16(q[ks][nt][i] & 0xffffu, p.a.q_f16)),
+                                   fabsf(value16(q[ks][nt][i] >> 16, p.a.q_f16))));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;  // floor(log2 top)
+        e = top > 0.f && top < INFINITY ? max(-100, min(e, 127)) : 13;
+        const float up = __uint_as_float(static_cast<uint32_t>(127 + 13 - e) << 23);
+        const float down = __uint_as_float(static_cast<uint32_t>(max(1, 127 + e - 13)) << 23);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            q[ks][nt][i] = pack16<false>(value16(q[ks][nt][i] & 0xffffu, p.a.q_f16) * up,
+                                         value16(q[ks][nt][i] >> 16, p.a.q_f16) * up);
+        factor[nt][0] = __shfl_sync(0xffffffffu, down, pair * 8) * p.a.scale_log2;
+        factor[nt][1] = __shfl_sync(0xffffffffu, down, pair * 8 + 4) * p.a.scale_log2;
+      } else {
+        factor[nt][0] = factor[nt][1] = p.a.scale_log2;
+      }
+    }
+
+    float m[NT][2], l[NT][2], o[DT][NT][4], vref = __uint_as_float(27u << 23);  // 2^-100
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[dt][nt][i] = 0.f;
+    }
+
+    for (int step = 0; step < seg; ++step) {
+      cp_wait<S - 2>();
+      __syncwarp();
+      const int key0 = here.tile * C::kTile + warp * C::kKeys;
+      const uint32_t mask = live[stage];
+      const uint32_t kb = ring + stage * C::kStage, vb = kb + C::kRowsBytes;
+      issue(stage == 0 ? S - 1 : stage - 1);
+      if (key0 < here.n) {
+        constexpr int kRsh = C::kRow >= 128 ? 0 : C::kRow == 64 ? 1 : 2;
+        constexpr int kMask = C::kChunks >= 8 ? 7 : C::kChunks - 1;
+        const auto chunk = [&](uint32_t base, int r, int col) {
+          return base + r * C::kRow + ((col ^ ((r >> kRsh) & kMask)) << 4);
+        };
+        // ---- S^T = K Q^T
+        float x[MT][NT][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[mt][nt][i] = 0.f;
+        const int lr = (lane & 7) + (lane & 8), lc = lane >> 4;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          if constexpr (C::kFp8) {
+#pragma unroll
+            for (int k2 = 0; k2 < KS / 2; ++k2) {
+              uint32_t w[4];
+              ldsm4(w, chunk(kb, mt * 16 + lr, 2 * k2 + lc));
+              const uint32_t a0[4] = {widen_lo(w[0]), widen_lo(w[1]), widen_hi(w[0]), widen_hi(w[1])};
+              const uint32_t a1[4] = {widen_lo(w[2]), widen_lo(w[3]), widen_hi(w[2]), widen_hi(w[3])};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma16816<false>(x[mt][nt], a0, q[2 * k2][nt][0], q[2 * k2][nt][1]);
+                mma16816<false>(x[mt][nt], a1, q[2 * k2 + 1][nt][0], q[2 * k2 + 1][nt][1]);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+              uint32_t w[4];
+              ldsm4(w, chunk(kb, mt * 16 + lr, 2 * ks + lc));
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                mma16816<C::kBf16>(x[mt][nt], w, q[ks][nt][0], q[ks][nt][1]);
+            }
+          }
+        }
+        // ---- scores in log2 units; what is not live is -inf
+        const float* scales = reinterpret_cast<const float*>(smem + warp * C::kRing + stage * C::kStage +
+                                                             2 * C::kRowsBytes);
+        float top[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) top[nt][0] = top[nt][1] = -INFINITY;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int r = mt * 16 + i * 8 + row;
+            const bool ok = (mask >> r) & 1;
+            float ks = 1.f;
+            if constexpr (C::kFp8) ks = scales[r];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                float& y = x[mt][nt][2 * i + j];
+                if constexpr (C::kFp8) y *= ks;
+                y = ok ? y * factor[nt][j] : -INFINITY;
+                top[nt][j] = fmaxf(top[nt][j], y);
+              }
+          }
+        if (p.scores) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int col = nt * 8 + pair * 2 + j;
+              if (col < cols) {
+                float* dst = p.scores + (static_cast<int64_t>(b) * p.a.Hq + hq0 + col) * p.score_pitch + key0;
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                  for (int i = 0; i < 2; ++i) {
+                    const int r = mt * 16 + i * 8 + row;
+                    if (key0 + r < here.n) dst[r] = x[mt][nt][2 * i + j];
+                  }
+              }
+            }
+        }
+        bool raise = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) raise |= top[nt][j] > m[nt][j] + kRescale;
+        if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float t = top[nt][j];
+              t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
+              t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
+              t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
+              t = fmaxf(t, m[nt][j]);
+              const float f = t == m[nt][j] ? 1.f : ex2(m[nt][j] - t);
+              m[nt][j] = t;
+              l[nt][j] *= f;
+#pragma unroll
+              for (int dt = 0; dt < DT; ++dt) {
+                o[dt][nt][j] *= f;
+                o[dt][nt][2 + j] *= f;
+              }
+            }
+        }
+        float vinv = 1.f;
+        if constexpr (C::kFp8) {
+          uint32_t v = __float_as_uint(scales[C::kKeys + my_key]) & 0x7fffffffu;
+          v = __reduce_max_sync(0xffffffffu, v);
+          if (v > __float_as_uint(vref)) {
+            // the next power of two, at most 2^126 (a scale above it is inf, NaN or as good as)
+            const float ref = __uint_as_float(min((v + 0x7fffffu) & 0x7f800000u, 253u << 23));
+            const float f = vref / ref;
+            vref = ref;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[dt][nt][i] *= f;
+          }
+          vinv = 1.f / vref;
+        }
+        // ---- O^T += V^T P^T
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          uint32_t pb[NT][2];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float e0 = ex2(x[mt][nt][2 * i] - finite_or_zero(m[nt][0]));
+              float e1 = ex2(x[mt][nt][2 * i + 1] - finite_or_zero(m[nt][1]));
+              l[nt][0] += e0;
+              l[nt][1] += e1;
+              if constexpr (C::kFp8) {
+                const float vs = scales[C::kKeys + mt * 16 + i * 8 + row] * vinv;
+                e0 *= vs;
+                e1 *= vs;
+              }
+              pb[nt][i] = transpose8(pack16<C::kBf16>(e0, e1));
+            }
+          if constexpr (C::kFp8) {
+#pragma unroll
+            for (int d2 = 0; d2 < DT / 2; ++d2) {
+              uint32_t w[4];
+              ldsm4t(w, chunk(vb, mt * 16 + lr, 2 * d2 + lc));
+#pragma unroll
+              for (int i = 0; i < 4; ++i) w[i] = __byte_perm(w[i], 0, 0x3120);
+              const uint32_t a0[4] = {widen_lo(w[0]), widen_hi(w[0]), widen_lo(w[1]), widen_hi(w[1])};
+              const uint32_t a1[4] = {widen_lo(w[2]), widen_hi(w[2]), widen_lo(w[3]), widen_hi(w[3])};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma16816<false>(o[2 * d2][nt], a0, pb[nt][0], pb[nt][1]);
+                mma16816<false>(o[2 * d2 + 1][nt], a1, pb[nt][0], pb[nt][1]);
+              }
+            }
+          } else {
+            const int vr = (lane & 7) + (lane >> 4) * 8, vc = (lane >> 3) & 1;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+              uint32_t w[4];
+              ldsm4t(w, chunk(vb, mt * 16 + vr, 2 * dt + vc));
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma16816<C::kBf16>(o[dt][nt], w, pb[nt][0], pb[nt][1]);
+            }
+          }
+        }
+      }
+      stage = stage == S - 1 ? 0 : stage + 1;
+      --left;
+      if (left > 0) here.next<C>(p);
+    }
+
+    // ---- the four warps' parts of this segment joined (in warp 0)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float t = l[nt][j];
+        t += __shfl_xor_sync(0xffffffffu, t, 4);
+        t += __shfl_xor_sync(0xffffffffu, t, 8);
+        t += __shfl_xor_sync(0xffffffffu, t, 16);
+        l[nt][j] = t;
+        if (row == 0) {
+          const int i = warp * NT * 8 + nt * 8 + pair * 2 + j;
+          sm_m[i] = m[nt][j];
+          sm_l[i] = t;
+        }
+      }
+    __syncthreads();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int i = nt * 8 + pair * 2 + j;
+        float top = sm_m[i], sum = 0.f;
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sm_m[w * NT * 8 + i]);
+        const float ref = finite_or_zero(top);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) sum += sm_l[w * NT * 8 + i] * ex2(sm_m[w * NT * 8 + i] - ref);
+        float f = ex2(m[nt][j] - ref);
+        if constexpr (C::kFp8) f *= vref;
+        m[nt][j] = top;
+        l[nt][j] = sum;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          o[dt][nt][j] *= f;
+          o[dt][nt][2 + j] *= f;
+        }
+      }
+    const auto put = [&](int buf) {
+#pragma unroll
+      for (int i = 0; i < C::kFrags; ++i) {
+        const float(&c)[4] = o[i / NT][i % NT];
+        join[(buf * C::kFrags + i) * 32 + lane] = make_float4(c[0], c[1], c[2], c[3]);
+      }
+    };
+    const auto take = [&](int buf) {
+#pragma unroll
+      for (int i = 0; i < C::kFrags; ++i) {
+        float(&c)[4] = o[i / NT][i % NT];
+        const float4 y = join[(buf * C::kFrags + i) * 32 + lane];
+        c[0] += y.x;
+        c[1] += y.y;
+        c[2] += y.z;
+        c[3] += y.w;
+      }
+    };
+    if (warp >= 2) put(warp - 2);
+    __syncthreads();
+    if (warp < 2) take(warp);
+    if (warp == 1) put(1);
+    __syncthreads();
+    if (warp == 0) {
+      take(1);
+      if (begins && ends) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int col = nt * 8 + pair * 2 + j;
+            if (col >= cols) continue;
+            const float inv = l[nt][j] == 0.f ? 0.f : 1.f / l[nt][j];
+            uint16_t* dst = p.a.out + b * p.a.o_seq + (hq0 + col) * p.a.o_head;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+              for (int half = 0; half < 2; ++half)
+                dst[dim_of<C::kFp8>(dt, row, half)] = round16(o[dt][nt][2 * half + j] * inv, p.a.q_f16);
+            if (row == 0) write_lse(p, b, hq0 + col, m[nt][j], l[nt][j]);
+          }
+      } else {
+        const int slot = blockIdx.x * 2 + (first_segment ? 0 : 1);
+#pragma unroll
+        for (int i = 0; i < C::kFrags; ++i) {
+          const float(&c)[4] = o[i / NT][i % NT];
+          p.part_o[(static_cast<int64_t>(slot) * C::kFrags + i) * 32 + lane] = make_float4(c[0], c[1], c[2], c[3]);
+        }
+        if (row == 0) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float* ml = p.part_ml + slot * 2 * NT * 8 + nt * 8 + pair * 2 + j;
+              ml[0] = m[nt][j];
+              ml[NT * 8] = l[nt][j];
+            }
+        }
+      }
+    }
+    if (!(begins && ends)) {
+      if (begins) {
+        cut.begun = b * items + head * p.groups + g0 / (NT * 8);
+        cut.begun_slot = first_segment ? 0 : 1;
+      } else {
+        cut.continued = b * items + head * p.groups + g0 / (NT * 8);
+      }
+    }
+    first_segment = false;
+  }
+  if (threadIdx.x == 0) p.cuts[blockIdx.x] = cut;
+}
+
+// Joins the partials of the item that CTA blockIdx.x of the main kernel began
+// and others continued: CTA blockIdx.x + 1, + 2, ... in order.
+template <int KV, int D, int NT>
+__global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const Params p) {
+  using C = Cfg<KV, D, NT>;
+  constexpr int kE = C::kFrags * 32;  // float4 elements of a partial
+  constexpr int kTeams = kJoinThreads > kE ? kJoinThreads / kE : 1;
+  extern __shared__ float factors[];  // (parts, NT * 8)
+  __shared__ float4 sums[kJoinThreads];
+  __shared__ float sm_inv[NT * 8];
+  __shared__ int count;
+  const Cut cut = p.cuts[blockIdx.x];
+  if (cut.begun < 0) return;
+  const int item = cut.begun, first_slot = blockIdx.x * 2 + cut.begun_slot;
+  if (threadIdx.x == 0) count = p.grid - blockIdx.x;
+  __syncthreads();
+  for (int c = blockIdx.x + 1 + threadIdx.x; c < p.grid; c += kJoinThreads)
+    if (p.cuts[c].continued != item) atomicMin(&count, c - static_cast<int>(blockIdx.x));
+  __syncthreads();
+  const int parts = count;
+  const auto slot_of = [&](int i) { return i == 0 ? first_slot : static_cast<int>((blockIdx.x + i) * 2); };
+  const int items = p.a.kv.heads * p.groups;
+  const int b = item / items, head = item % items / p.groups, g0 = item % p.groups * NT * 8;
+  const int cols = min(NT * 8, p.G - g0), hq0 = head * p.G + g0;
+  // one warp per column: the maximum, the sum, every partial's factor
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp < NT * 8) {
+    float m = -INFINITY, l = 0.f;
+    for (int i = lane; i < parts; i += 32) m = fmaxf(m, p.part_ml[slot_of(i) * 2 * NT * 8 + warp]);
+#pragma unroll
+    for (int s = 16; s > 0; s /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
+    const float ref = finite_or_zero(m);
+    for (int i = lane; i < parts; i += 32) {
+      const float* ml = p.part_ml + slot_of(i) * 2 * NT * 8 + warp;
+      const float f = ex2(ml[0] - ref);
+      factors[i * NT * 8 + warp] = f;
+      l += ml[NT * 8] * f;
+    }
+#pragma unroll
+    for (int s = 16; s > 0; s /= 2) l += __shfl_xor_sync(0xffffffffu, l, s);
+    if (lane == 0) {
+      sm_inv[warp] = l == 0.f ? 0.f : 1.f / l;
+      if (warp < cols) write_lse(p, b, hq0 + warp, m, l);
+    }
+  }
+  __syncthreads();
+  const int team = threadIdx.x / kE;
+  for (int e = threadIdx.x % kE; e < kE; e += kJoinThreads) {
+    const int ln = e % 32, nt = e / 32 % NT, dt = e / 32 / NT;
+    const int c0 = nt * 8 + (ln & 3) * 2;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = team; i < parts; i += kTeams) {
+      const float4 y = p.part_o[static_cast<int64_t>(slot_of(i)) * kE + e];
+      const float f0 = factors[i * NT * 8 + c0], f1 = factors[i * NT * 8 + c0 + 1];
+      s.x += y.x * f0;
+      s.y += y.y * f1;
+      s.z += y.z * f0;
+      s.w += y.w * f1;
+    }
+    if constexpr (kTeams > 1) {
+      sums[threadIdx.x] = s;
+      __syncthreads();
+      if (team > 0) return;
+#pragma unroll
+      for (int i = 1; i < kTeams; ++i) {
+        const float4 y = sums[threadIdx.x + i * kE];
+        s.x += y.x;
+        s.y += y.y;
+        s.z += y.z;
+        s.w += y.w;
+      }
+    }
+    const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int col = c0 + (i & 1);
+      if (col < cols)
+        p.a.out[b * p.a.o_seq + (hq0 + col) * p.a.o_head + dim_of<C::kFp8>(dt, ln >> 2, i >> 1)] =
+            round16(v[i] * sm_inv[col], p.a.q_f16);
+    }
+  }
+}
+
+// Every key's weights, summed over the query heads of its KV head in order.
+__global__ void __launch_bounds__(256) decode_weights_kernel(const Params p) {
+  const int h = blockIdx.y, b = blockIdx.z;
+  const int n = table_length(p.a.t, p.a.kv.page_size, b, p.a.status);
+  const int64_t row = static_cast<int64_t>(b) * p.a.Hq + h * p.G;
+  const float* scores = p.scores + row * p.score_pitch;
+  const float* lse2 = p.lse2 + row;
+  float* dst = p.a.weights.w + b * p.a.weights.s_seq + h * p.a.weights.s_head;
+  for (int j = blockIdx.x * 256 + threadIdx.x; j < n; j += gridDim.x * 256) {
+    float w = 0.f;
+#pragma unroll 4
+    for (int g = 0; g < p.G; ++g) {
+      const float y = __ldg(lse2 + g);
+      w += ex2(__ldg(scores + static_cast<int64_t>(g) * p.score_pitch + j) - finite_or_zero(y));
+    }
+    dst[j] += w;
+  }
+}
+
+constexpr int kMaxDevices = 64;
+
+int current_device() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < kMaxDevices ? dev : 0;
+}
+
+int sm_count(int dev) {
+  static std::atomic<int> known[kMaxDevices];
+  int n = known[dev].load(std::memory_order_relaxed);
+  if (n == 0 && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess)
+    known[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+// Column blocks of 8 query heads that a group of G heads is given: two at most
+// (a group of more than 16 heads takes several passes over its keys).
+int column_blocks(int G) { return G > 8 ? 2 : 1; }
+
+struct Workspace {
+  size_t part_ml, cuts, lse2, scores, total;
+  int pitch;
+  Workspace(const PagedPool& kv, int B, int Hq, int table_pages, bool weights) {
+    const size_t heads = static_cast<size_t>(B) * Hq;
+    const int nt = column_blocks(Hq / kv.heads);
+    const auto next = [this](size_t bytes) {
+      const size_t at = total;
+      total += (bytes + 127) / 128 * 128;
+      return at;
+    };
+    total = 0;
+    pitch = (table_pages * kv.page_size + 31) / 32 * 32;
+    next(static_cast<size_t>(kMaxCtas) * 2 * (kv.D / 16) * nt * 512);  // part_o, at 0
+    part_ml = next(static_cast<size_t>(kMaxCtas) * 2 * 2 * nt * 8 * 4);
+    cuts = next(kMaxCtas * sizeof(Cut));
+    lse2 = next(weights ? heads * 4 : 0);
+    scores = next(weights ? heads * pitch * 4 : 0);
+  }
+};
+
+template <int KV, int D, int NT>
+cudaError_t launch(Params p, cudaStream_t st) {
+  using C = Cfg<KV, D, NT>;
+  static std::atomic<int> known[kMaxDevices];  // CTAs an SM holds, once this device is set up
+  const int dev = current_device();
+  int per_sm = known[dev].load(std::memory_order_relaxed);
+  if (per_sm == 0) {
+    cudaError_t e = cudaFuncSetAttribute(decode_kernel<KV, D, NT>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (e != cudaSuccess) return e;
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, decode_kernel<KV, D, NT>, kThreads, C::kSmem);
+    if (e != cudaSuccess) return e;
+    e = cudaFuncSetAttribute(decode_join_kernel<KV, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kMaxCtas * NT * 8 * 4);
+    if (e != cudaSuccess) return e;
+    if (per_sm < 1) per_sm = 1;
+    known[dev].store(per_sm, std::memory_order_relaxed);
+  }
+  p.grid = sm_count(dev) * per_sm < kMaxCtas ? sm_count(dev) * per_sm : kMaxCtas;
+  if (p.grid <= 0) return cudaErrorInvalidDevice;
+  decode_kernel<KV, D, NT><<<p.grid, kThreads, C::kSmem, st>>>(p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  decode_join_kernel<KV, D, NT><<<p.grid, kJoinThreads, p.grid * NT * 8 * 4, st>>>(p);
+  return cudaGetLastError();
+}
+
+template <int KV, int D>
+cudaError_t launch_nt(const Params& p, int nt, cudaStream_t st) {
+  return nt == 1 ? launch<KV, D, 1>(p, st) : launch<KV, D, 2>(p, st);
+}
+
+template <int KV>
+cudaError_t launch_d(const Params& p, int nt, cudaStream_t st) {
+  switch (p.a.kv.D) {
+    case 32: return launch_nt<KV, 32>(p, nt, st);
+    case 64: return launch_nt<KV, 64>(p, nt, st);
+    case 128: return launch_nt<KV, 128>(p, nt, st);
+    case 256: return launch_nt<KV, 256>(p, nt, st);
+    default: return cudaErrorInvalidValue;
+  }
+}
 
 }  // namespace
 
@@ -137,26 +893,34 @@ size_t paged_decode_workspace(const PagedPool& kv, int B, int Hq, int table_page
 }
 
 cudaError_t launch_paged_decode(const PagedDecodeArgs& a, cudaStream_t st) {
-  const Workspace ws(a.kv, a.t.B, a.Hq, a.t.pages, a.weights.w != nullptr);
+  const bool weights = a.weights.w != nullptr;
+  const Workspace ws(a.kv, a.t.B, a.Hq, a.t.pages, weights);
   char* base = static_cast<char*>(a.workspace);
-  float* part = reinterpret_cast<float*>(base + ws.part);
-  float* lse2 = reinterpret_cast<float*>(base + ws.lse2);
-  float* scores = a.weights.w ? reinterpret_cast<float*>(base + ws.scores) : nullptr;
-  const int cap = a.t.pages * a.kv.page_size;
-  const dim3 grid(kSplits, a.Hq, a.t.B);
-  switch (a.kv.D) {
-    case 32: decode_kernel<32><<<grid, 32, 0, st>>>(a, part, scores, cap); break;
-    case 64: decode_kernel<64><<<grid, 32, 0, st>>>(a, part, scores, cap); break;
-    case 128: decode_kernel<128><<<grid, 32, 0, st>>>(a, part, scores, cap); break;
-    case 256: decode_kernel<256><<<grid, 32, 0, st>>>(a, part, scores, cap); break;
-    default: return cudaErrorInvalidValue;
+  Params p{};
+  p.a = a;
+  p.G = a.Hq / a.kv.heads;
+  const int nt = column_blocks(p.G);
+  p.groups = (p.G + nt * 8 - 1) / (nt * 8);
+  p.shift = -1;
+  for (int s = 0; s < 31; ++s)
+    if (a.kv.page_size == 1 << s) p.shift = s;
+  p.score_pitch = ws.pitch;
+  p.part_o = reinterpret_cast<float4*>(base);
+  p.part_ml = reinterpret_cast<float*>(base + ws.part_ml);
+  p.cuts = reinterpret_cast<Cut*>(base + ws.cuts);
+  p.lse2 = weights ? reinterpret_cast<float*>(base + ws.lse2) : nullptr;
+  p.scores = weights ? reinterpret_cast<float*>(base + ws.scores) : nullptr;
+  cudaError_t e = cudaErrorInvalidValue;
+  switch (a.kv.dtype) {
+    case kKvBf16: e = launch_d<kKvBf16>(p, nt, st); break;
+    case kKvF16: e = launch_d<kKvF16>(p, nt, st); break;
+    case kKvE4m3: e = launch_d<kKvE4m3>(p, nt, st); break;
   }
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  decode_join_kernel<<<dim3(a.Hq, a.t.B), a.kv.D, 0, st>>>(a, part, lse2, a.kv.D);
-  e = cudaGetLastError();
-  if (e != cudaSuccess || !scores || cap == 0) return e;
-  decode_weights_kernel<<<dim3((cap + 255) / 256, a.kv.heads, a.t.B), 256, 0, st>>>(a, scores, lse2, cap);
+  const int cap = a.t.pages * a.kv.page_size;
+  if (e != cudaSuccess || !weights || cap == 0) return e;
+  // enough CTAs for the SMs, at most one per 256 positions
+  const int rows = a.kv.heads * a.t.B, want = (16 * sm_count(current_device()) + rows - 1) / rows, most = (cap + 255) / 256;
+  decode_weights_kernel<<<dim3(want < most ? want : most, a.kv.heads, a.t.B), 256, 0, st>>>(p);
   return cudaGetLastError();
 }
 
