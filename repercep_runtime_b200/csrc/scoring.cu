@@ -2,108 +2,466 @@
 // row of logits.
 //
 // With m = max_v x_v, l = sum_v e^(x_v - m) and lse = m + log l:
-//   logprob = x_token - lse
+//   logprob = (x_token - m) - log l        (not x_token - lse, which cancels
+//                                           where |m| is large)
 //   entropy = log l - (sum_v e^(x_v - m) (x_v - m)) / l
-//   top     = the `top` largest x_v - lse, ties to the lowest index.
+//   top     = the `top` largest x_v, ties to the lowest index.
 // A row whose every logit is -inf has entropy 0 and log probabilities -inf;
 // a NaN or +inf in a row makes its sums NaN.
+//
+// One pass over the logits, bound by HBM (and, for 16-bit logits, not far from
+// the exp rate: one MUFU operation an element).  A thread keeps a reference
+// value, moved only when a value exceeds it by 6.9 (2^10 in e^x), and sums e^(x - ref) and
+// its product with x - ref in fp32; the maximum is not needed exactly.
+// Alternatives cost the pass nothing but a running maximum: each thread leaves
+// the maxima of its segments (32 to a few hundred values) in shared memory.
+// Afterwards the k-th largest of 128 group maxima is a lower bound of the k-th
+// largest value, and the few segments that reach it are read again (from L2).
+// Few rows are split over a cluster of CTAs, joined through distributed shared
+// memory: one launch, no workspace.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "internal.h"
 #include "paged.h"
+#include "ptx.cuh"
 
 namespace rp {
 namespace {
 
-constexpr int kScoreThreads = 512;
+namespace cg = cooperative_groups;
 
-__device__ __forceinline__ float logit(const void* row, int64_t i, int dtype) {
-  if (dtype == 2) return static_cast<const float*>(row)[i];
-  const uint16_t u = static_cast<const uint16_t*>(row)[i];
-  return dtype == 1 ? __half2float(__ushort_as_half(u)) : __uint_as_float(static_cast<uint32_t>(u) << 16);
-}
+constexpr int kT = 256;              // threads of a CTA
+constexpr int kU = 4;                // 16-byte vectors a thread has in flight
+constexpr int kGroups = 128;         // groups whose maxima bound the k-th value
+constexpr int kSegments = 16;        // segments of a thread, at most
+constexpr int kCandidates = 2048;    // values kept for the selection
+constexpr int kMaxCluster = 8;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kHeadroom = 6.9f;    // the reference may lie 2^10 below a value
 
-// Order of alternatives as one integer: larger value first, then lower index.
-// NaN is above +inf, -0 equals 0.
-__device__ __forceinline__ uint64_t rank_key(float x, int i) {
+// Order of values as one integer: NaN above +inf, -0 equal to 0; and back.
+__device__ __forceinline__ uint32_t value_key(float x) {
   uint32_t u = __float_as_uint(x);
-  if (x != x) u = 0xffffffffu;
-  else if (u == 0x80000000u) u = 0x80000000u;
-  else u = (u & 0x80000000u) ? ~u : u | 0x80000000u;
-  return (static_cast<uint64_t>(u) << 32) | (0xffffffffu - static_cast<uint32_t>(i));
+  if (x != x) return 0xffffffffu;
+  if (u == 0x80000000u) u = 0;
+  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
+}
+// Alternatives in order: larger value first, then lower index.
+__device__ __forceinline__ uint64_t rank_key(float x, int i) {
+  return (static_cast<uint64_t>(value_key(x)) << 32) | (0xffffffffu - static_cast<uint32_t>(i));
 }
 
-template <typename T, typename F>
-__device__ T block_reduce(T x, T* buf, F f) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+// Element types: DT is an rp_dtype.
+template <int DT>
+struct Type {
+  static constexpr int kVec = DT == 2 ? 4 : 8;  // elements of a 16-byte vector
+  static constexpr int kSize = 16 / kVec;
+  static constexpr uint32_t kNegInf = DT == 2 ? 0xFF800000u : DT == 1 ? 0xFC00FC00u : 0xFF80FF80u;
+  __device__ static __forceinline__ float at(const void* p, int64_t i) {
+    if constexpr (DT == 2) return __ldg(static_cast<const float*>(p) + i);
+    const uint16_t u = __ldg(static_cast<const uint16_t*>(p) + i);
+    return DT == 1 ? __half2float(__ushort_as_half(u)) : __uint_as_float(static_cast<uint32_t>(u) << 16);
+  }
+  // The two values of word w of a 16-bit vector.
+  __device__ static __forceinline__ float2 pair(uint32_t w) {
+    if constexpr (DT == 1) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+  // Larger of two words' values (element-wise when 16-bit); NaN wins.
+  __device__ static __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    uint32_t y;
+    if constexpr (DT == 0) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+    else if constexpr (DT == 1) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+    else y = __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b)));
+    return y;
+  }
+  __device__ static __forceinline__ float value(uint32_t w) {
+    if constexpr (DT == 2) return __uint_as_float(w);
+    const float2 v = pair(w);
+    return max_nan(v.x, v.y);
+  }
+};
+
+// Sums over a set of values relative to ref: l = sum e^(x - ref), s = sum
+// e^(x - ref) log2(e) (x - ref).
+struct Sums {
+  float ref, l, s;
+  // The same sums relative to `to` (not below ref's rounding of them).
+  __device__ __forceinline__ void move(float to) {
+    if (l == 0.f) {
+      s = 0.f;
+    } else {
+      const float y = ((ref == -INFINITY ? 0.f : ref) - to) * kLog2e, f = ex2(y);
+      s = f * (s + l * fmaxf(y, -1000.f));
+      l *= f;
+    }
+    ref = to;
+  }
+};
+__device__ __forceinline__ Sums joined(Sums a, Sums b) {
+  const float to = fmaxf(a.ref, b.ref), ref = to == -INFINITY ? 0.f : to;
+  a.move(ref);
+  b.move(ref);
+  return Sums{to, a.l + b.l, a.s + b.s};
+}
+
+struct Shared {
+  Sums warp_sums[kT / 32];
+  Sums sums;                        // of this CTA
+  uint32_t groups[kGroups];         // keys of the group maxima
+  uint64_t best[kMaxTop];           // this CTA's alternatives
+  uint64_t merged[kMaxCluster * kMaxTop];
+  int count, picked;
+  uint32_t bound;
+};
+
+// The `k` largest of n different keys, in order, to out[0..k) (n >= k).  keys
+// may be reordered.  All threads of the CTA.
+__device__ void select_top(uint64_t* keys, int n, int k, uint64_t* out, Shared& sh) {
+  __syncthreads();
+  if (n > kT) {
+    // the k-th largest, bit by bit, and what lies at or above it to the front
+    uint64_t thr = 0;
+    for (int bit = 63; bit >= 0; --bit) {
+      const uint64_t t = thr | (1ull << bit);
+      int c = 0;
+      for (int i = threadIdx.x; i < n; i += kT) c += keys[i] >= t;
+      c = __reduce_add_sync(0xffffffffu, c);
+      if (threadIdx.x == 0) sh.picked = 0;
+      __syncthreads();
+      if ((threadIdx.x & 31) == 0) atomicAdd(&sh.picked, c);
+      __syncthreads();
+      const bool enough = sh.picked >= k;
+      __syncthreads();
+      if (enough) thr = t;
+    }
+    if (threadIdx.x == 0) sh.picked = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kT)
+      if (keys[i] >= thr) out[atomicAdd(&sh.picked, 1)] = keys[i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < k; i += kT) keys[i] = out[i];
+    n = k;
+    __syncthreads();
+  }
+  if (threadIdx.x < n) {
+    const uint64_t key = keys[threadIdx.x];
+    int rank = 0;
+    for (int i = 0; i < n; ++i) rank += keys[i] > key;
+    if (rank < k) out[rank] = key;
+  }
+  __syncthreads();
+}
+
+// One row per cluster; the CTAs of a cluster take equal parts of it.
+template <int DT>
+__global__ void __launch_bounds__(kT, 4) score_kernel(const ScoreArgs a, int per_segment) {
+  using E = Type<DT>;
+  constexpr int kVec = E::kVec;
+  extern __shared__ uint64_t dynamic[];  // with alternatives: candidates, then segment maxima
+  __shared__ Shared sh;
+  uint64_t* cand = dynamic;
+  float* segs = reinterpret_cast<float*>(dynamic + kCandidates);
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int parts = static_cast<int>(cluster.num_blocks()), part = static_cast<int>(cluster.block_rank());
+  const int r = blockIdx.x / parts, t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  const int V = a.vocab, top = a.top;
+  const char* row = static_cast<const char*>(a.logits) + r * a.stride * E::kSize;
+
+  // The row as vectors that start at 16-byte boundaries: vector v holds
+  // elements v * kVec - shift + i, of which the first and last may lack some.
+  const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15) / E::kSize;
+  const uint4* base = reinterpret_cast<const uint4*>(row - shift * E::kSize);
+  const int vectors = (V + shift + kVec - 1) / kVec;
+  const int v0 = static_cast<int>(static_cast<int64_t>(vectors) * part / parts);
+  const int v1 = static_cast<int>(static_cast<int64_t>(vectors) * (part + 1) / parts);
+  const int inner0 = shift ? 1 : 0, inner1 = (V + shift) / kVec;  // whole vectors
+  const auto edge = [&](int v) {  // a vector with elements missing: -inf there
+    uint32_t w[4] = {E::kNegInf, E::kNegInf, E::kNegInf, E::kNegInf};
 #pragma unroll
-  for (int s = 16; s > 0; s /= 2) x = f(x, __shfl_xor_sync(0xffffffffu, x, s));
+    for (int i = 0; i < kVec; ++i) {
+      const int e = v * kVec - shift + i;
+      if (e < 0 || e >= V) continue;
+      if constexpr (DT == 2) {
+        w[i] = __ldg(reinterpret_cast<const uint32_t*>(row) + e);
+      } else {
+        const uint32_t u = __ldg(reinterpret_cast<const uint16_t*>(row) + e);
+        w[i / 2] = i % 2 ? (w[i / 2] & 0xffffu) | (u << 16) : (w[i / 2] & 0xffff0000u) | u;
+      }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  };
+  const auto load = [&](int v) {
+    if (v >= inner0 && v < inner1) return __ldcs(base + v);
+    return edge(v);
+  };
+
+  // ---- the pass
+  Sums mine{-INFINITY, 0.f, 0.f};
+  float seg = -INFINITY, best = -INFINITY;
+  int in_seg = 0, n_seg = 0;
+  uint64_t l2 = 0, s2 = 0;
+  for (int v = v0 + t; v < v1; v += kU * kT) {
+    uint4 x[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u)
+      x[u] = v + u * kT < v1 ? load(v + u * kT) : make_uint4(E::kNegInf, E::kNegInf, E::kNegInf, E::kNegInf);
+    uint32_t m = x[0].x;
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      m = E::larger(m, E::larger(x[u].x, x[u].y));
+      m = E::larger(m, E::larger(x[u].z, x[u].w));
+    }
+    const float big = E::value(m);
+    if (big > mine.ref + kHeadroom) {
+      float p, q;
+      unpack_f32x2(l2, p, q);
+      mine.l = p + q;
+      unpack_f32x2(s2, p, q);
+      mine.s = p + q;
+      mine.move(big);
+      l2 = pack_f32x2(mine.l, 0.f);
+      s2 = pack_f32x2(mine.s, 0.f);
+    }
+    seg = max_nan(seg, big);
+    if (top > 0 && ++in_seg == per_segment) {
+      segs[n_seg++ * kT + t] = seg;
+      best = max_nan(best, seg);
+      seg = -INFINITY;
+      in_seg = 0;
+    }
+    const float ref = mine.ref == -INFINITY ? 0.f : mine.ref;
+    const uint64_t nref = pack_f32x2(-ref, -ref), scale = pack_f32x2(kLog2e, kLog2e);
+    const auto two = [&](float x0, float x1) {
+      const uint64_t y = fmul2(fadd2(pack_f32x2(x0, x1), nref), scale);
+      float y0, y1;
+      unpack_f32x2(y, y0, y1);
+      const uint64_t e = pack_f32x2(ex2(y0), ex2(y1));
+      l2 = fadd2(l2, e);
+      // e is 0 where the clamp acts (-inf logits)
+      s2 = ffma2(e, pack_f32x2(fmaxf(y0, -1000.f), fmaxf(y1, -1000.f)), s2);
+    };
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+      if constexpr (DT == 2) {
+        two(__uint_as_float(w[0]), __uint_as_float(w[1]));
+        two(__uint_as_float(w[2]), __uint_as_float(w[3]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = E::pair(w[i]);
+          two(f.x, f.y);
+        }
+      }
+    }
+  }
+  {
+    float p, q;
+    unpack_f32x2(l2, p, q);
+    mine.l = p + q;
+    unpack_f32x2(s2, p, q);
+    mine.s = p + q;
+  }
+#pragma unroll
+  for (int s = 16; s > 0; s /= 2)
+    mine = joined(mine, Sums{__shfl_xor_sync(0xffffffffu, mine.ref, s), __shfl_xor_sync(0xffffffffu, mine.l, s),
+                             __shfl_xor_sync(0xffffffffu, mine.s, s)});
+  if (lane == 0) sh.warp_sums[warp] = mine;
+
+  // ---- this part's alternatives
+  const int have = min(V, v1 * kVec - shift) - max(0, v0 * kVec - shift);  // its elements
+  const int k = min(top, max(have, 0));
+  if (k > 0) {
+    if (in_seg > 0) {
+      segs[n_seg++ * kT + t] = seg;
+      best = max_nan(best, seg);
+    }
+    float g = best;
+#pragma unroll
+    for (int s = 1; s < kT / kGroups; s *= 2) g = max_nan(g, __shfl_xor_sync(0xffffffffu, g, s));
+    if (t % (kT / kGroups) == 0) sh.groups[t / (kT / kGroups)] = value_key(g);
+    if (t == 0) {
+      sh.count = 0;
+      sh.bound = 0;
+    }
+    __syncthreads();
+    if (t < kGroups) {
+      const uint32_t key = sh.groups[t];
+      int above = 0;
+      for (int i = 0; i < kGroups; ++i) above += sh.groups[i] > key || (sh.groups[i] == key && i < t);
+      if (above == k - 1) sh.bound = key;
+    }
+    __syncthreads();
+    // candidates: every value at or above the bound; `strict`: above it
+    const auto collect = [&](uint32_t bound, bool strict) {
+      for (int i = 0; i < n_seg; ++i) {
+        const uint32_t sk = value_key(segs[i * kT + t]);
+        if (strict ? sk <= bound : sk < bound) continue;
+        for (int j = 0; j < per_segment * kU; ++j) {
+          const int v = v0 + t + (i * per_segment * kU + j) * kT;
+          if (v >= v1) break;
+          for (int c = 0; c < kVec; ++c) {
+            const int e = v * kVec - shift + c;
+            if (e < 0 || e >= V) continue;
+            const float x = E::at(row, e);
+            const uint32_t key = value_key(x);
+            if (strict ? key <= bound : key < bound) continue;
+            const int at = atomicAdd(&sh.count, 1);
+            if (at < kCandidates) cand[at] = rank_key(x, e);
+          }
+        }
+      }
+      __syncthreads();
+    };
+    uint32_t bound = sh.bound;
+    collect(bound, false);
+    int n = sh.count;
+    __syncthreads();
+    // Too many: the values above the bound alone.  Are these too many as well,
+    // the k-th largest of those at hand is a higher bound.
+    while (n > kCandidates) {
+      if (t == 0) sh.count = 0;
+      __syncthreads();
+      collect(bound, true);
+      n = sh.count;
+      __syncthreads();
+      if (n > kCandidates) {
+        select_top(cand, kCandidates, k, sh.best, sh);
+        bound = static_cast<uint32_t>(sh.best[k - 1] >> 32);
+        if (t == 0) sh.count = 0;
+        __syncthreads();
+        collect(bound, false);
+        n = sh.count;
+        __syncthreads();
+      } else if (n < k) {
+        // the lowest indices among the values equal to the bound
+        const int e0 = max(0, v0 * kVec - shift), e1 = min(V, v1 * kVec - shift);
+        int need = k - n;
+        for (int e = e0; e < e1 && need > 0; e += kT) {
+          const bool tie = e + t < e1 && value_key(E::at(row, e + t)) == bound;
+          const uint32_t votes = __ballot_sync(0xffffffffu, tie);
+          if (lane == 0) sh.groups[warp] = __popc(votes);
+          __syncthreads();
+          int before = __popc(votes & ((1u << lane) - 1)), all = 0;
+          for (int w = 0; w < kT / 32; ++w) {
+            if (w < warp) before += sh.groups[w];
+            all += sh.groups[w];
+          }
+          if (tie && before < need) cand[n + before] = rank_key(key_value(bound), e + t);
+          n += min(all, need);
+          need -= min(all, need);
+          __syncthreads();
+        }
+      }
+    }
+    select_top(cand, n, k, sh.best, sh);
+  }
   __syncthreads();
-  if (lane == 0) buf[warp] = x;
-  __syncthreads();
-  x = buf[0];
-  for (int w = 1; w < kScoreThreads / 32; ++w) x = f(x, buf[w]);
-  return x;
+  if (t == 0) {
+    Sums all = sh.warp_sums[0];
+    for (int w = 1; w < kT / 32; ++w) all = joined(all, sh.warp_sums[w]);
+    sh.sums = all;
+    sh.picked = k;
+  }
+
+  // ---- the parts joined by the cluster's first CTA
+  uint64_t* best_keys = sh.best;
+  if (parts > 1) {
+    cluster.sync();
+    if (part == 0 && top > 0) {
+      int n = 0;
+      for (int i = 0; i < parts; ++i) {
+        const Shared* other = cluster.map_shared_rank(&sh, i);
+        const int m = other->picked;
+        for (int j = t; j < m; j += kT) sh.merged[n + j] = other->best[j];
+        n += m;
+      }
+      __syncthreads();
+      select_top(sh.merged, n, top, cand, sh);
+      best_keys = cand;
+    }
+  } else {
+    __syncthreads();
+  }
+  if (part == 0) {
+    Sums all = sh.sums;
+    for (int i = 1; i < parts; ++i) all = joined(all, cluster.map_shared_rank(&sh, i)->sums);
+    const bool nothing = all.l == 0.f;  // every logit -inf
+    const float ref = all.ref == -INFINITY ? 0.f : all.ref, logl = logf(all.l);
+    if (t == 0) {
+      const int64_t token = a.tokens[r];
+      float lp = 0.f;
+      if (token >= V) {
+        atomicCAS(a.status, 0, kStatusBadToken);
+        lp = __int_as_float(0x7fc00000);
+      } else if (token >= 0) {
+        lp = nothing ? -INFINITY : (E::at(row, token) - ref) - logl;
+      }
+      a.logprobs[r] = lp;
+      a.entropy[r] = nothing ? 0.f : logl - kLn2 * (all.s / all.l);
+    }
+    for (int i = t; i < top; i += kT) {
+      const uint64_t key = best_keys[i];
+      a.top_ids[static_cast<int64_t>(r) * top + i] = 0xffffffffu - static_cast<uint32_t>(key);
+      a.top_logprobs[static_cast<int64_t>(r) * top + i] =
+          nothing ? -INFINITY : (key_value(static_cast<uint32_t>(key >> 32)) - ref) - logl;
+    }
+  }
+  if (parts > 1) cluster.sync();  // the others' shared memory is read until here
 }
 
-// One CTA a row: maximum, then the sums, then one pass per alternative.
-__global__ void __launch_bounds__(kScoreThreads) score_kernel(const ScoreArgs a) {
-  __shared__ float fbuf[kScoreThreads / 32];
-  __shared__ uint64_t kbuf[kScoreThreads / 32];
-  const int r = blockIdx.x, size = a.dtype == 2 ? 4 : 2;
-  const void* row = static_cast<const char*>(a.logits) + r * a.stride * size;
-  const auto fmax2 = [](float x, float y) { return (x != x || x > y) ? x : y; };
-  const auto add = [](float x, float y) { return x + y; };
-  float m = -INFINITY;
-  for (int i = threadIdx.x; i < a.vocab; i += kScoreThreads) m = fmax2(logit(row, i, a.dtype), m);
-  m = block_reduce(m, fbuf, fmax2);
-  const float ref = m == -INFINITY ? 0.f : m;
-  float l = 0.f, s = 0.f;
-  for (int i = threadIdx.x; i < a.vocab; i += kScoreThreads) {
-    const float d = logit(row, i, a.dtype) - ref, e = expf(d);
-    l += e;
-    if (e != 0.f) s += e * d;
-  }
-  l = block_reduce(l, fbuf, add);
-  s = block_reduce(s, fbuf, add);
-  const float logl = logf(l);
-  if (threadIdx.x == 0) {
-    const int64_t t = a.tokens[r];
-    float lp = 0.f;
-    if (t >= a.vocab) {
-      atomicCAS(a.status, 0, kStatusBadToken);
-      lp = __int_as_float(0x7fc00000);
-    } else if (t >= 0) {
-      // (x - m) - log l, not x - lse: the latter cancels where |m| is large
-      lp = m == -INFINITY ? -INFINITY : (logit(row, t, a.dtype) - ref) - logl;
-    }
-    a.logprobs[r] = lp;
-    a.entropy[r] = m == -INFINITY ? 0.f : logl - s / l;
-  }
-  uint64_t last = ~0ull;
-  for (int k = 0; k < a.top; ++k) {
-    uint64_t best = 0;
-    for (int i = threadIdx.x; i < a.vocab; i += kScoreThreads) {
-      const uint64_t key = rank_key(logit(row, i, a.dtype), i);
-      if (key < last && key > best) best = key;
-    }
-    best = block_reduce(best, kbuf, [](uint64_t x, uint64_t y) { return x > y ? x : y; });
-    last = best;
-    if (threadIdx.x == 0) {
-      const int64_t i = 0xffffffffu - static_cast<uint32_t>(best);
-      a.top_ids[static_cast<int64_t>(r) * a.top + k] = i;
-      a.top_logprobs[static_cast<int64_t>(r) * a.top + k] =
-          m == -INFINITY ? -INFINITY : (logit(row, i, a.dtype) - ref) - logl;
-    }
-  }
+template <int DT>
+cudaError_t launch(const ScoreArgs& a, cudaStream_t st) {
+  // CTAs of a row: enough for four CTAs an SM, with at least 1024 vectors each.
+  constexpr int kVec = Type<DT>::kVec;
+  const int64_t vectors = static_cast<int64_t>(a.vocab) / kVec + 2;
+  int parts = 1;
+  while (parts < kMaxCluster && static_cast<int64_t>(a.rows) * parts * 2 <= 148 * 4 &&
+         vectors / (parts * 2) >= kT)
+    parts *= 2;
+  const int64_t batches = (vectors / parts + 1 + kU * kT - 1) / (kU * kT);  // of a thread
+  const int per_segment = static_cast<int>((batches + kSegments - 1) / kSegments);
+  const int64_t segments = (batches + per_segment - 1) / per_segment;
+  const size_t smem = a.top > 0 ? kCandidates * 8 + static_cast<size_t>(segments) * kT * 4 : 0;
+  if (static_cast<int64_t>(a.rows) * parts > 0x7FFFFFFF) return cudaErrorInvalidValue;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(a.rows) * parts);
+  cfg.blockDim = dim3(kT);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = parts;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, score_kernel<DT>, a, per_segment);
 }
 
 }  // namespace
 
 cudaError_t launch_token_logprobs(const ScoreArgs& a, cudaStream_t st) {
-  score_kernel<<<a.rows, kScoreThreads, 0, st>>>(a);
-  return cudaGetLastError();
+  return a.dtype == 2 ? launch<2>(a, st) : a.dtype == 1 ? launch<1>(a, st) : launch<0>(a, st);
 }
 
 }  // namespace rp
