@@ -1,10 +1,16 @@
 // Paged key-value cache: append and evict (see include/repercep_b200.h).
+#include <cooperative_groups.h>
+
+#include <atomic>
+
 #include "internal.h"
 #include "paged.h"
 #include "quant_common.cuh"
 
 namespace rp {
 namespace {
+
+namespace cg = cooperative_groups;
 
 constexpr int kAppendThreads = 256;
 
@@ -91,111 +97,301 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelectThreads = 1024;
-
-__device__ __forceinline__ int block_sum(int x, int* buf) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  x = __reduce_add_sync(0xffffffffu, x);
-  __syncthreads();
-  if (lane == 0) buf[warp] = x;
-  __syncthreads();
-  return __reduce_add_sync(0xffffffffu, lane < kSelectThreads / 32 ? buf[lane] : 0);
+// The weight of a key (0 for -0, one NaN for all).
+__device__ __forceinline__ float key_weight(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
 }
 
-// Exclusive prefix of x over the block's threads; *total: the sum.
-__device__ __forceinline__ int block_prefix(int x, int* buf, int* total) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int y = x;
-#pragma unroll
-  for (int s = 1; s < 32; s *= 2) {
-    const int z = __shfl_up_sync(0xffffffffu, y, s);
-    if (lane >= s) y += z;
-  }
-  __syncthreads();
-  if (lane == 31) buf[warp] = y;
-  __syncthreads();
-  int before = 0, all = 0;
-  for (int w = 0; w < kSelectThreads / 32; ++w) {
-    if (w < warp) before += buf[w];
-    all += buf[w];
-  }
-  *total = all;
-  return before + y - x;
-}
+// ---- selection
+//
+// One cluster of CTAs per (sequence, KV head): each CTA keeps the keys of its
+// slice of the row in shared memory, and the threshold (the want-th largest
+// key) is found in at most three passes over them, 11, 11 and 10 bits at a
+// time, with a histogram per CTA that every CTA of the cluster adds up through
+// distributed shared memory: sums of 8 bins first, then the bins of one such
+// sum.  (All 2048 bins at once take 4500 cycles a pass; 8 bits at a time do not
+// work either: weights share few exponents, and the adds to a few bins, or the
+// matching of lanes that avoids them, take most of the time.)  Two passes more
+// count and place what is kept in order, so ties at the threshold go to the
+// lowest positions.  Reads each weight from HBM once; bound by the latency of
+// its few dependent passes, which the split over a cluster shortens.
+constexpr int kSelThreads = 512;
+constexpr int kSelWarps = kSelThreads / 32;
+constexpr int kSelBatch = 8;  // keys of a thread in flight
+constexpr int kBins = 2048;
+constexpr int kCoarse = kBins / 8;
+constexpr int kSelCluster = 8;         // CTAs of a row, at most
+constexpr int kSliceAim = 8192;        // positions of a CTA that a larger cluster is not taken for
+constexpr int kSliceHeld = 44 * 1024;  // positions of a CTA held in shared memory, at most
 
-// Positions to keep, one CTA per (sequence, head): the threshold is the
-// largest key with at least `want` candidates at or above it, found bit by
-// bit; ties at it go to the lowest positions.
-__global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const EvictArgs a) {
-  __shared__ int buf[kSelectThreads / 32];
-  const int h = blockIdx.x, b = blockIdx.y, H = a.kv.heads;
+struct SelectShared {
+  int4 hist[3][kBins / 4];
+  int4 coarse[3][kCoarse / 4];
+  int4 all[kSelCluster][kCoarse / 4];
+  int above[kSelWarps], ties[kSelWarps];  // of each warp's run
+  int part_above, part_ties;              // of this CTA's slice
+  int scan[kSelWarps];
+  int digit, left, whole;
+};
+
+// HELD: every slice fits the shared memory; else keys are made from the
+// weights again in each pass.
+template <bool HELD>
+__global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictArgs a) {
+  extern __shared__ uint32_t slice[];
+  __shared__ SelectShared sh;
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int parts = static_cast<int>(cluster.num_blocks()), part = static_cast<int>(cluster.block_rank());
+  const int h = blockIdx.x / parts, b = blockIdx.y, H = a.kv.heads;
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
   const int n = table_length(a.t, a.kv.page_size, b, a.status);
   const int keep = min(n, a.budget);
   const float* w = a.weights.w + b * a.weights.s_seq + h * a.weights.s_head;
   int32_t* kept = a.kept + (static_cast<int64_t>(b) * H + h) * a.budget;
   const int64_t out_cap = static_cast<int64_t>(a.out_pages) * a.kv.page_size;
   float* wo = a.weights_out + (static_cast<int64_t>(b) * H + h) * out_cap;
-  if (h == 0 && threadIdx.x == 0) a.lengths_out[b] = keep;
-  const int older = n > a.budget ? n - a.recent : n;   // candidates [0, older)
-  const int want = n > a.budget ? a.budget - a.recent : n;
+  const int stride = parts * kSelThreads, first = part * kSelThreads + t;
+  // candidates [0, older), of which `want` stay; what is behind them stays whole
+  const bool cut = n > a.budget;
+  const int older = cut ? n - a.recent : n, want = cut ? a.budget - a.recent : n;
+  const bool search = cut && want > 0;  // the same in the whole cluster
+  const int per = (older + parts - 1) / parts, i0 = min(older, part * per);
+  const int count = search ? min(older, i0 + per) - i0 : 0;
+  if (HELD) {  // all of a thread's weights in flight at once
+    for (int i = t; i < count; i += kSelThreads)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(slice + i)), "l"(w + i0 + i) : "memory");
+  }
+  if (blockIdx.x == 0 && t == 0) a.lengths_out[b] = keep;
+  for (int i = keep + first; i < a.budget; i += stride) kept[i] = -1;
+  for (int64_t i = keep + first; i < out_cap; i += stride) wo[i] = 0.f;
+  for (int i = (cut ? older : 0) + first; i < n; i += stride) {
+    kept[want - (cut ? older : want) + i] = i;
+    wo[want - (cut ? older : want) + i] = w[i];
+  }
+  if (!search) return;
+
+  for (int i = t; i < 3 * kBins / 4; i += kSelThreads) (&sh.hist[0][0])[i] = make_int4(0, 0, 0, 0);
+  if (HELD) {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    // a thread makes keys of the weights that it brought in itself
+#pragma unroll 4
+    for (int i = t; i < count; i += kSelThreads) slice[i] = weight_key(__uint_as_float(slice[i]));
+  }
+  __syncthreads();
+  const auto key_at = [&](int i) { return HELD ? slice[i] : weight_key(__ldg(w + i0 + i)); };
+
   uint32_t thr = 0;
-  int above = 0;  // candidates above thr
-  if (want < older) {
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t t = thr | (1u << bit);
-      int c = 0;
-      for (int i = threadIdx.x; i < older; i += kSelectThreads) c += weight_key(w[i]) >= t;
-      if (block_sum(c, buf) >= want) thr = t;
+  int left = want;  // rank of the threshold among the keys that share its known bits
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const int bits = pass == 2 ? 10 : 11, shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    int* hist = reinterpret_cast<int*>(sh.hist[pass]);
+    for (int base = warp * 32; base < count; base += kSelBatch * kSelThreads) {
+      uint32_t key[kSelBatch];
+      bool in[kSelBatch];
+#pragma unroll
+      for (int u = 0; u < kSelBatch; ++u) {
+        const int i = base + u * kSelThreads + lane;
+        key[u] = i < count ? key_at(i) : 0;
+        // equal known bits (all, in the first pass)
+        in[u] = i < count && (pass == 0 || (key[u] ^ thr) >> (shift + bits) == 0);
+      }
+#pragma unroll
+      for (int u = 0; u < kSelBatch; ++u) {
+        // lanes of the first such lane's bin are counted by one add: rows with many equal weights
+        const uint32_t live = __ballot_sync(0xffffffffu, in[u]);
+        if (live == 0) continue;
+        const int bin = (key[u] >> shift) & ((1 << bits) - 1), lead = __ffs(live) - 1;
+        const int bin0 = __shfl_sync(0xffffffffu, bin, lead);
+        const uint32_t same = __ballot_sync(0xffffffffu, in[u] && bin == bin0);
+        if (in[u] && (bin != bin0 || lane == lead)) atomicAdd(&hist[bin], bin == bin0 ? __popc(same) : 1);
+      }
     }
-    int c = 0;
-    for (int i = threadIdx.x; i < older; i += kSelectThreads) c += weight_key(w[i]) > thr;
-    above = block_sum(c, buf);
-  }
-  int out = 0, ties = want - above;  // ties still to take
-  for (int i0 = 0; i0 < n; i0 += kSelectThreads) {
-    const int i = i0 + threadIdx.x;
-    const uint32_t key = i < older ? weight_key(w[i]) : 0;
-    const bool all = want >= older;
-    const bool tie = !all && i < older && key == thr;
-    int n_tie = 0, n_out = 0;
-    const int tie_at = block_prefix(tie, buf, &n_tie);
-    const bool take = i < n && (i >= older || all || key > thr || (tie && tie_at < ties));
-    const int at = out + block_prefix(take, buf, &n_out);
-    if (take) {
-      kept[at] = i;
-      wo[at] = w[i];
+    __syncthreads();
+    if (t < kCoarse) {
+      const int4 x = sh.hist[pass][2 * t], y = sh.hist[pass][2 * t + 1];
+      reinterpret_cast<int*>(sh.coarse[pass])[t] = x.x + x.y + x.z + x.w + y.x + y.y + y.z + y.w;
     }
-    ties -= min(n_tie, ties);
-    out += n_out;
+    if (parts > 1) cluster.sync();
+    else __syncthreads();
+    if (t < parts * (kCoarse / 4)) {
+      const int q = t / (kCoarse / 4), quad = t % (kCoarse / 4);
+      sh.all[q][quad] = cluster.map_shared_rank(&sh, q)->coarse[pass][quad];
+    }
+    __syncthreads();
+    // a sum of 8 bins a thread, from the top: the one in which the running count reaches `left`
+    int c = 0, before = 0;
+    if (t < kCoarse) {
+      for (int i = 0; i < parts; ++i) c += reinterpret_cast<const int*>(sh.all[i])[kCoarse - 1 - t];
+      before = c;
+#pragma unroll
+      for (int s = 1; s < 32; s *= 2) {
+        const int x = __shfl_up_sync(0xffffffffu, before, s);
+        if (lane >= s) before += x;
+      }
+      if (lane == 31) sh.scan[warp] = before;
+    }
+    __syncthreads();
+    if (t < kCoarse) {
+      before -= c;
+#pragma unroll
+      for (int i = 0; i < kCoarse / 32; ++i) before += i < warp ? sh.scan[i] : 0;
+      if (before < left && before + c >= left) {
+        sh.digit = kCoarse - 1 - t;
+        sh.left = left - before;
+      }
+    }
+    __syncthreads();
+    // its bins, by one warp: lane i sums bin 7 - i % 8 over two of the CTAs
+    if (warp == 0) {
+      const int group = sh.digit, rest = sh.left, bin = group * 8 + 7 - (lane & 7);
+      int n0 = 0, n1 = 0;
+      const int q0 = lane >> 3, q1 = q0 + 4;
+      if (q0 < parts) n0 = reinterpret_cast<const int*>(cluster.map_shared_rank(&sh, q0)->hist[pass])[bin];
+      if (q1 < parts) n1 = reinterpret_cast<const int*>(cluster.map_shared_rank(&sh, q1)->hist[pass])[bin];
+      int m = n0 + n1;
+      m += __shfl_xor_sync(0xffffffffu, m, 8);
+      m += __shfl_xor_sync(0xffffffffu, m, 16);
+      int run = m;
+#pragma unroll
+      for (int s = 1; s < 8; s *= 2) {
+        const int x = __shfl_up_sync(0xffffffffu, run, s, 8);
+        if ((lane & 7) >= s) run += x;
+      }
+      __syncwarp();
+      if (lane < 8 && run - m < rest && run >= rest) {
+        sh.digit = bin;
+        sh.left = rest - (run - m);
+        sh.whole = run == rest;
+      }
+    }
+    __syncthreads();
+    thr |= static_cast<uint32_t>(sh.digit) << shift;
+    left = sh.left;  // among the keys of this bin; after the last pass, the ties to take
+    if (sh.whole) {  // all of the bin stays: what is above the key below it (no key is 0)
+      thr -= 1;
+      left = 0;
+      break;
+    }
   }
-  for (int i = keep + threadIdx.x; i < a.budget; i += kSelectThreads) kept[i] = -1;
-  for (int64_t i = keep + threadIdx.x; i < out_cap; i += kSelectThreads) wo[i] = 0.f;
+
+  // ---- places: each warp a run of the slice, in order
+  const int run = (count + kSelWarps - 1) / kSelWarps, r0 = min(count, warp * run), r1 = min(count, r0 + run);
+  int above = 0, ties = 0;
+#pragma unroll 8
+  for (int i = r0 + lane; i < r1; i += 32) {
+    const uint32_t key = key_at(i);
+    above += key > thr;
+    ties += key == thr;
+  }
+  above = __reduce_add_sync(0xffffffffu, above);
+  ties = __reduce_add_sync(0xffffffffu, ties);
+  if (lane == 0) {
+    sh.above[warp] = above;
+    sh.ties[warp] = ties;
+  }
+  __syncthreads();
+  int at_above = 0, at_ties = 0;
+#pragma unroll
+  for (int q = 0; q < kSelWarps; ++q) {
+    at_above += q < warp ? sh.above[q] : 0;
+    at_ties += q < warp ? sh.ties[q] : 0;
+  }
+  if (parts > 1) {
+    if (t == kSelThreads - 1) {  // of the last warp: the whole slice
+      sh.part_above = at_above + above;
+      sh.part_ties = at_ties + ties;
+    }
+    cluster.sync();
+    // lane q reads what CTA q's slice holds
+    int2 p = make_int2(0, 0);
+    if (lane < part) {
+      const SelectShared* other = cluster.map_shared_rank(&sh, lane);
+      p = make_int2(other->part_above, other->part_ties);
+    }
+    at_above += __reduce_add_sync(0xffffffffu, p.x);
+    at_ties += __reduce_add_sync(0xffffffffu, p.y);
+    cluster.barrier_arrive();  // the others' shared memory is read until here
+  }
+  for (int base = r0; base < r1; base += 32 * kSelBatch) {
+    uint32_t gt[kSelBatch], eq[kSelBatch];
+    uint32_t key[kSelBatch];
+#pragma unroll
+    for (int u = 0; u < kSelBatch; ++u) {
+      const int i = base + u * 32 + lane;
+      key[u] = i < r1 ? key_at(i) : 0;
+      gt[u] = __ballot_sync(0xffffffffu, i < r1 && key[u] > thr);
+      eq[u] = __ballot_sync(0xffffffffu, i < r1 && key[u] == thr);
+    }
+#pragma unroll
+    for (int u = 0; u < kSelBatch; ++u) {
+      const uint32_t below = (1u << lane) - 1;
+      const int tie = at_ties + __popc(eq[u] & below);  // ties before this one
+      if (((gt[u] >> lane) & 1) || (((eq[u] >> lane) & 1) && tie < left)) {
+        const int at = at_above + __popc(gt[u] & below) + min(tie, left);
+        kept[at] = i0 + base + u * 32 + lane;
+        wo[at] = key_weight(key[u]);
+      }
+      at_above += __popc(gt[u]);
+      at_ties += __popc(eq[u]);
+    }
+  }
+  if (parts > 1) cluster.barrier_wait();
 }
 
-// Rows to their new places, one warp per kept row.
-__global__ void __launch_bounds__(256) evict_move_kernel(const EvictArgs a, int row_bytes) {
+// ---- move
+//
+// Kept rows to their new places: a warp takes 8 rows, their places found by 8
+// lanes, with K and V of all of them in flight before the first store.
+constexpr int kMoveRows = 8;
+constexpr int kMoveWarps = 8;
+
+template <int ROW>  // bytes of a row
+__global__ void __launch_bounds__(kMoveWarps * 32) evict_move_kernel(const EvictArgs a) {
+  constexpr int kLanes = ROW / 16;                               // lanes of a row
+  constexpr int kTurns = kMoveRows * kLanes > 32 ? kMoveRows * kLanes / 32 : 1;  // vectors of K a lane
+  constexpr int kAtOnce = 32 / kLanes;                           // rows of a turn
   const int lane = threadIdx.x & 31;
-  const int j = blockIdx.x * 8 + (threadIdx.x >> 5), h = blockIdx.y, b = blockIdx.z, H = a.kv.heads;
-  if (j >= a.budget) return;
-  const int p = a.kept[(static_cast<int64_t>(b) * H + h) * a.budget + j];
-  if (p < 0) return;
-  const int32_t* from_row = a.t.table + b * a.t.stride;
-  const int32_t* to_row = a.out_table + b * a.out_stride;
-  const int64_t from = row_offset(a.kv, from_row, p, h, a.status);
-  const int64_t to = row_offset(a.kv, to_row, j, h, a.status);
-  if (from < 0 || to < 0) return;
+  const int j0 = (blockIdx.x * kMoveWarps + (threadIdx.x >> 5)) * kMoveRows, h = blockIdx.y, b = blockIdx.z;
+  const int H = a.kv.heads;
+  const int j = j0 + lane;
+  const int p = lane < kMoveRows && j < a.budget ? a.kept[(static_cast<int64_t>(b) * H + h) * a.budget + j] : -1;
+  int64_t from = -1, to = -1;
+  if (p >= 0) {
+    const int32_t* from_row = a.t.table + b * a.t.stride;
+    const int32_t* to_row = a.out_table + b * a.out_stride;
+    from = row_offset(a.kv, from_row, p, h, a.status);
+    to = row_offset(a.kv, to_row, j, h, a.status);
+    if (from < 0 || to < 0) {
+      to = -1;
+    } else if (a.kv.ks) {
+      const int64_t i = scale_index(a.kv, from_row, p, h), o = scale_index(a.kv, to_row, j, h);
+      const float ks = a.kv.ks[i], vs = a.kv.vs[i];
+      a.kv.ks[o] = ks;
+      a.kv.vs[o] = vs;
+    }
+  }
   const int size = a.kv.dtype == kKvE4m3 ? 1 : 2;
-  for (int c = lane * 16; c < row_bytes; c += 512) {
-    const uint4 k = *reinterpret_cast<const uint4*>(a.kv.k + from * size + c);
-    const uint4 v = *reinterpret_cast<const uint4*>(a.kv.v + from * size + c);
-    *reinterpret_cast<uint4*>(a.kv.k + to * size + c) = k;
-    *reinterpret_cast<uint4*>(a.kv.v + to * size + c) = v;
+  const int col = lane % kLanes * 16;
+  uint4 k[kTurns], v[kTurns];
+  int64_t dst[kTurns];
+#pragma unroll
+  for (int i = 0; i < kTurns; ++i) {
+    const int r = i * kAtOnce + lane / kLanes;
+    const int64_t src = __shfl_sync(0xffffffffu, from, r % 32) * size + col;
+    const int64_t d = __shfl_sync(0xffffffffu, to, r % 32);
+    dst[i] = d < 0 || r >= kMoveRows ? -1 : d * size + col;
+    if (dst[i] >= 0) {
+      k[i] = __ldcs(reinterpret_cast<const uint4*>(a.kv.k + src));
+      v[i] = __ldcs(reinterpret_cast<const uint4*>(a.kv.v + src));
+    }
   }
-  if (a.kv.ks && lane == 0) {
-    const int64_t i = scale_index(a.kv, from_row, p, h), o = scale_index(a.kv, to_row, j, h);
-    a.kv.ks[o] = a.kv.ks[i];
-    a.kv.vs[o] = a.kv.vs[i];
-  }
+#pragma unroll
+  for (int i = 0; i < kTurns; ++i)
+    if (dst[i] >= 0) {
+      *reinterpret_cast<uint4*>(a.kv.k + dst[i]) = k[i];
+      *reinterpret_cast<uint4*>(a.kv.v + dst[i]) = v[i];
+    }
 }
 
 }  // namespace
@@ -216,11 +412,47 @@ cudaError_t launch_paged_append(const AppendArgs& a, cudaStream_t st) {
 }
 
 cudaError_t launch_paged_evict(const EvictArgs& a, cudaStream_t st) {
-  evict_select_kernel<<<dim3(a.kv.heads, a.t.B), kSelectThreads, 0, st>>>(a);
-  cudaError_t e = cudaGetLastError();
+  const int64_t cap = static_cast<int64_t>(a.t.pages) * a.kv.page_size;
+  int parts = 1;
+  // a larger cluster while the slices are long and the GPU holds all CTAs at once
+  while (parts < kSelCluster && cap > static_cast<int64_t>(parts) * kSliceAim &&
+         static_cast<int64_t>(a.kv.heads) * a.t.B * parts * 2 <= 148 * 4)
+    parts *= 2;
+  const int64_t per = (cap + parts - 1) / parts;
+  const bool held = per <= kSliceHeld;
+  if (static_cast<int64_t>(a.kv.heads) * parts > 0x7FFFFFFF) return cudaErrorInvalidValue;
+  static std::atomic<bool> ready[kMaxDevices];
+  const int dev = current_device();
+  if (!ready[dev].load(std::memory_order_relaxed)) {
+    const cudaError_t e = cudaFuncSetAttribute(evict_select_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               kSliceHeld * 4);
+    if (e != cudaSuccess) return e;
+    ready[dev].store(true, std::memory_order_relaxed);
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(a.kv.heads * parts, a.t.B);
+  cfg.blockDim = dim3(kSelThreads);
+  cfg.dynamicSmemBytes = held ? static_cast<size_t>(per) * 4 : 0;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = parts;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = held ? cudaLaunchKernelEx(&cfg, evict_select_kernel<true>, a)
+                       : cudaLaunchKernelEx(&cfg, evict_select_kernel<false>, a);
   if (e != cudaSuccess) return e;
-  const dim3 grid((a.budget + 7) / 8, a.kv.heads, a.t.B);
-  evict_move_kernel<<<grid, 256, 0, st>>>(a, a.kv.D * (a.kv.dtype == kKvE4m3 ? 1 : 2));
+  constexpr int kRows = kMoveRows * kMoveWarps;
+  const dim3 grid((a.budget + kRows - 1) / kRows, a.kv.heads, a.t.B);
+  switch (a.kv.D * (a.kv.dtype == kKvE4m3 ? 1 : 2)) {
+    case 32: evict_move_kernel<32><<<grid, kMoveWarps * 32, 0, st>>>(a); break;
+    case 64: evict_move_kernel<64><<<grid, kMoveWarps * 32, 0, st>>>(a); break;
+    case 128: evict_move_kernel<128><<<grid, kMoveWarps * 32, 0, st>>>(a); break;
+    case 256: evict_move_kernel<256><<<grid, kMoveWarps * 32, 0, st>>>(a); break;
+    case 512: evict_move_kernel<512><<<grid, kMoveWarps * 32, 0, st>>>(a); break;
+    default: return cudaErrorInvalidValue;
+  }
   return cudaGetLastError();
 }
 

@@ -109,6 +109,13 @@ struct ScoreArgs {
 };
 cudaError_t launch_token_logprobs(const ScoreArgs& a, cudaStream_t st);
 
+// Per-device settings of the launchers are kept for this many devices.
+constexpr int kMaxDevices = 64;
+inline int current_device() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < kMaxDevices ? dev : 0;
+}
+
 #ifdef __CUDACC__
 // Length of sequence b, held to what its page table can address.
 __device__ __forceinline__ int table_length(const PagedTable& t, int page_size, int b, int* status) {

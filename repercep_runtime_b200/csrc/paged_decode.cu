@@ -803,13 +803,6 @@ __global__ void __launch_bounds__(256) decode_weights_kernel(const Params p) {
   }
 }
 
-constexpr int kMaxDevices = 64;
-
-int current_device() {
-  int dev = 0;
-  return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < kMaxDevices ? dev : 0;
-}
-
 int sm_count(int dev) {
   static std::atomic<int> known[kMaxDevices];
   int n = known[dev].load(std::memory_order_relaxed);
