@@ -99,6 +99,8 @@ int rp_paged_append(const rp_paged_kv* kv, const void* k_new, const void* v_new,
   if (a.kv.dtype != RP_KV_E4M3 && (a.kv.dtype == RP_KV_F16) != (in_dtype == RP_DTYPE_F16))
     return set_last_error(RP_ERR_INVALID, "new rows and a 16-bit cache must share a dtype");
   if (tokens < 0) return set_last_error(RP_ERR_INVALID, "tokens is negative");
+  if (static_cast<int64_t>(tokens) * a.kv.heads > 0x7FFFFFFF - 65536)
+    return set_last_error(RP_ERR_UNSUPPORTED, "more than 2^31 new rows");
   if (!starts && tokens != B)
     return set_last_error(RP_ERR_INVALID, "%d new tokens for %d sequences without starts", tokens, B);
   if (B == 0) return RP_OK;

@@ -15,77 +15,124 @@ namespace cg = cooperative_groups;
 constexpr int kAppendThreads = 256;
 
 // New rows into the cache.  A row of D 16-bit values is D / 8 16-byte
-// vectors, one a thread, so a warp holds 256 / D rows; K and V of a row are
-// loaded together.  Rows are numbered (token, head), as the input has them.
-// e4m3: the amax of a row is a shuffle over its D / 8 lanes, and the steps
-// are the quantizer's (quant_common.cuh), so the bytes are those of the
-// row-wise quantizer.  Reads 4 D bytes and writes 2 D (or 4 D) a row.
-template <int D, bool E4M3, bool F16>
+// vectors, one a thread, so a warp holds 256 / D rows; a CTA takes a run of U *
+// 2048 / D rows, numbered (token, head) as the input has them.  While the K and
+// V vectors of a thread's U rows are on their way, one thread per token finds
+// its sequence, page and slot (done by every thread for every row, this took
+// twice the time of the rest).  e4m3: the amax of a row is a shuffle over its D
+// / 8 lanes, and the steps are the quantizer's (quant_common.cuh), so the bytes
+// are those of the row-wise quantizer.  Bound by HBM: reads 4 D bytes and
+// writes 2 D (or 4 D) a row.
+template <int D, bool E4M3, bool F16, int U>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs a) {
-  constexpr int kLanes = D / 8;  // threads a row
-  const int64_t gid = static_cast<int64_t>(blockIdx.x) * kAppendThreads + threadIdx.x;
-  const int H = a.kv.heads, B = a.t.B;
-  if (gid < B) {
-    const int n = table_length(a.t, a.kv.page_size, static_cast<int>(gid), a.status);
-    const int64_t add = a.starts ? static_cast<int64_t>(a.starts[gid + 1]) - a.starts[gid] : 1;
-    a.lengths_out[gid] = static_cast<int>(n + (add > 0 ? add : 0));
-  }
-  const int64_t r = gid / kLanes;
-  const int c = static_cast<int>(gid % kLanes);
-  if (r >= static_cast<int64_t>(a.tokens) * H) return;  // whole rows: the shuffles below stay in a row
-  const int t = static_cast<int>(r / H), h = static_cast<int>(r % H);
-  int b = t, first = t;
-  if (a.starts) {  // the sequence with starts[b] <= t < starts[b + 1]
-    if (t < a.starts[0] || t >= a.starts[B]) return;
-    int lo = 0, hi = B - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) / 2;
-      if (a.starts[mid] <= t) lo = mid;
-      else hi = mid - 1;
-    }
-    b = lo;
-    first = a.starts[b];
-  }
-  const int64_t pos = static_cast<int64_t>(table_length(a.t, a.kv.page_size, b, a.status)) + (t - first);
-  if (pos < 0 || pos >= static_cast<int64_t>(a.t.pages) * a.kv.page_size) {
-    if (c == 0) atomicCAS(a.status, 0, kStatusBadLength);
-    return;
-  }
-  const int p = static_cast<int>(pos);
-  const int32_t* row = a.t.table + b * a.t.stride;
-  const int64_t off = row_offset(a.kv, row, p, h, a.status);
-  if (off < 0) return;
-  const uint4 k = __ldg(reinterpret_cast<const uint4*>(a.k_new + t * a.k_tok + h * a.k_head) + c);
-  const uint4 v = __ldg(reinterpret_cast<const uint4*>(a.v_new + t * a.v_tok + h * a.v_head) + c);
-  if constexpr (E4M3) {
-    uint32_t mk = quant::absmax8(k), mv = quant::absmax8(v);
-    const unsigned lanes = kLanes == 32 ? 0xffffffffu : ((1u << kLanes) - 1) << (threadIdx.x & 31 & ~(kLanes - 1));
+  constexpr int kLanes = D / 8;                     // threads a row
+  constexpr int kAtOnce = kAppendThreads / kLanes;  // rows a CTA takes at once
+  constexpr int kTokens = kAtOnce * U;              // tokens of a CTA, at most
+  __shared__ int64_t offset[kTokens];               // of (token, head 0), -1: left out
+  __shared__ int64_t scale_at[E4M3 ? kTokens : 1];
+  __shared__ int64_t weight_at[kTokens];
+  const uint32_t H = a.kv.heads, B = a.t.B;
+  const int c = threadIdx.x % kLanes;
+  const uint32_t rows = static_cast<uint32_t>(a.tokens) * H, begin = blockIdx.x * kTokens;
+  const uint32_t r0 = begin + threadIdx.x / kLanes;
+  uint4 k[U], v[U];
+  uint32_t tok[U], head[U];
 #pragma unroll
-    for (int s = kLanes / 2; s > 0; s /= 2) {
-      mk = max(mk, __shfl_xor_sync(lanes, mk, s));
-      mv = max(mv, __shfl_xor_sync(lanes, mv, s));
+  for (int u = 0; u < U; ++u) {
+    const uint32_t r = r0 + u * kAtOnce;
+    tok[u] = r / H;
+    head[u] = r - tok[u] * H;
+    if (r < rows) {
+      k[u] = __ldcs(reinterpret_cast<const uint4*>(a.k_new + tok[u] * a.k_tok + head[u] * a.k_head) + c);
+      v[u] = __ldcs(reinterpret_cast<const uint4*>(a.v_new + tok[u] * a.v_tok + head[u] * a.v_head) + c);
     }
-    const float sk = quant::scale_from_amax_bits<F16>(mk), sv = quant::scale_from_amax_bits<F16>(mv);
-    reinterpret_cast<uint2*>(a.kv.k + off)[c] = quant::quant8_any<F16>(k, __frcp_rn(sk), isfinite(sk));
-    reinterpret_cast<uint2*>(a.kv.v + off)[c] = quant::quant8_any<F16>(v, __frcp_rn(sv), isfinite(sv));
-    if (c == 0) {
-      const int64_t i = scale_index(a.kv, row, p, h);
-      a.kv.ks[i] = sk;
-      a.kv.vs[i] = sv;
-    }
-  } else {
-    reinterpret_cast<uint4*>(a.kv.k + 2 * off)[c] = k;
-    reinterpret_cast<uint4*>(a.kv.v + 2 * off)[c] = v;
   }
-  if (a.weights.w && c == 0) a.weights.w[b * a.weights.s_seq + h * a.weights.s_head + p] = 0.f;
+  for (uint32_t i = blockIdx.x * kAppendThreads + threadIdx.x; i < B; i += gridDim.x * kAppendThreads) {
+    const int n = table_length(a.t, a.kv.page_size, i, a.status);
+    const int64_t add = a.starts ? static_cast<int64_t>(a.starts[i + 1]) - a.starts[i] : 1;
+    a.lengths_out[i] = static_cast<int>(n + (add > 0 ? add : 0));
+  }
+  const uint32_t t0 = begin / H, t1 = (min(begin + kTokens, rows) + H - 1) / H;  // the run's tokens
+  for (uint32_t i = threadIdx.x; begin < rows && i < t1 - t0; i += kAppendThreads) {
+    const int t = static_cast<int>(t0 + i);
+    int b = t, first = t;
+    bool ok = true;
+    if (a.starts) {  // the sequence with starts[b] <= t < starts[b + 1]
+      ok = t >= __ldg(a.starts) && t < __ldg(a.starts + B);
+      int lo = 0, hi = static_cast<int>(B) - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (__ldg(a.starts + mid) <= t) lo = mid;
+        else hi = mid - 1;
+      }
+      b = lo;
+      first = __ldg(a.starts + b);
+    }
+    int64_t off = -1;
+    if (ok) {
+      const int64_t pos = static_cast<int64_t>(table_length(a.t, a.kv.page_size, b, a.status)) + (t - first);
+      if (pos < 0 || pos >= static_cast<int64_t>(a.t.pages) * a.kv.page_size) {
+        atomicCAS(a.status, 0, kStatusBadLength);
+      } else {
+        const int p = static_cast<int>(pos);
+        const int32_t* row = a.t.table + b * a.t.stride;
+        off = row_offset(a.kv, row, p, 0, a.status);
+        if (E4M3 && off >= 0) scale_at[i] = scale_index(a.kv, row, p, 0);
+        weight_at[i] = b * a.weights.s_seq + p;
+      }
+    }
+    offset[i] = off;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (r0 + u * kAtOnce >= rows) return;  // whole rows: the shuffles below stay in a row
+    const uint32_t i = tok[u] - t0;
+    if (offset[i] < 0) continue;
+    const int64_t off = offset[i] + head[u] * a.kv.s_head;
+    if constexpr (E4M3) {
+      uint32_t mk = quant::absmax8(k[u]), mv = quant::absmax8(v[u]);
+      const unsigned lanes =
+          kLanes == 32 ? 0xffffffffu : ((1u << (kLanes % 32)) - 1) << (threadIdx.x & 31 & ~(kLanes - 1));
+#pragma unroll
+      for (int s = kLanes / 2; s > 0; s /= 2) {
+        mk = max(mk, __shfl_xor_sync(lanes, mk, s));
+        mv = max(mv, __shfl_xor_sync(lanes, mv, s));
+      }
+      const float sk = quant::scale_from_amax_bits<F16>(mk), sv = quant::scale_from_amax_bits<F16>(mv);
+      reinterpret_cast<uint2*>(a.kv.k + off)[c] = quant::quant8_any<F16>(k[u], __frcp_rn(sk), isfinite(sk));
+      reinterpret_cast<uint2*>(a.kv.v + off)[c] = quant::quant8_any<F16>(v[u], __frcp_rn(sv), isfinite(sv));
+      if (c == 0) {
+        const int64_t at = scale_at[i] + static_cast<int64_t>(head[u]) * a.kv.page_size;
+        a.kv.ks[at] = sk;
+        a.kv.vs[at] = sv;
+      }
+    } else {
+      reinterpret_cast<uint4*>(a.kv.k + 2 * off)[c] = k[u];
+      reinterpret_cast<uint4*>(a.kv.v + 2 * off)[c] = v[u];
+    }
+    if (a.weights.w && c == 0) a.weights.w[weight_at[i] + head[u] * a.weights.s_head] = 0.f;
+  }
 }
 
-template <int D>
-cudaError_t append_d(const AppendArgs& a, unsigned grid, cudaStream_t st) {
-  if (a.kv.dtype != kKvE4m3) append_kernel<D, false, false><<<grid, kAppendThreads, 0, st>>>(a);
-  else if (a.in_f16) append_kernel<D, true, true><<<grid, kAppendThreads, 0, st>>>(a);
-  else append_kernel<D, true, false><<<grid, kAppendThreads, 0, st>>>(a);
+template <int D, int U>
+cudaError_t append_u(const AppendArgs& a, cudaStream_t st) {
+  constexpr int kRows = kAppendThreads / (D / 8) * U;  // of a CTA
+  const int64_t rows = static_cast<int64_t>(a.tokens) * a.kv.heads;
+  int64_t grid = (rows + kRows - 1) / kRows;
+  if (grid < 1) grid = 1;  // lengths_out
+  const unsigned g = static_cast<unsigned>(grid);
+  if (a.kv.dtype != kKvE4m3) append_kernel<D, false, false, U><<<g, kAppendThreads, 0, st>>>(a);
+  else if (a.in_f16) append_kernel<D, true, true, U><<<g, kAppendThreads, 0, st>>>(a);
+  else append_kernel<D, true, false, U><<<g, kAppendThreads, 0, st>>>(a);
   return cudaGetLastError();
+}
+
+// Four rows a thread once the GPU is full all the same (148 SMs of 2048 threads).
+template <int D>
+cudaError_t append_d(const AppendArgs& a, cudaStream_t st) {
+  const int64_t threads = static_cast<int64_t>(a.tokens) * a.kv.heads * (D / 8);
+  return threads >= 4LL * 148 * 2048 ? append_u<D, 4>(a, st) : append_u<D, 1>(a, st);
 }
 
 // Weights order: a key is larger when the weight is; -0 equals 0 and any NaN
@@ -397,16 +444,11 @@ __global__ void __launch_bounds__(kMoveWarps * 32) evict_move_kernel(const Evict
 }  // namespace
 
 cudaError_t launch_paged_append(const AppendArgs& a, cudaStream_t st) {
-  const int64_t threads = static_cast<int64_t>(a.tokens) * a.kv.heads * (a.kv.D / 8);
-  const int64_t grid = ((threads > a.t.B ? threads : a.t.B) + kAppendThreads - 1) / kAppendThreads;
-  if (grid == 0) return cudaSuccess;
-  if (grid > 0x7FFFFFFF) return cudaErrorInvalidValue;
-  const unsigned g = static_cast<unsigned>(grid);
   switch (a.kv.D) {
-    case 32: return append_d<32>(a, g, st);
-    case 64: return append_d<64>(a, g, st);
-    case 128: return append_d<128>(a, g, st);
-    case 256: return append_d<256>(a, g, st);
+    case 32: return append_d<32>(a, st);
+    case 64: return append_d<64>(a, st);
+    case 128: return append_d<128>(a, st);
+    case 256: return append_d<256>(a, st);
     default: return cudaErrorInvalidValue;
   }
 }
