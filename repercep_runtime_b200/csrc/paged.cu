@@ -19,10 +19,13 @@ constexpr int kAppendThreads = 256;
 // 2048 / D rows, numbered (token, head) as the input has them.  While the K and
 // V vectors of a thread's U rows are on their way, one thread per token finds
 // its sequence, page and slot (done by every thread for every row, this took
-// twice the time of the rest).  e4m3: the amax of a row is a shuffle over its D
-// / 8 lanes, and the steps are the quantizer's (quant_common.cuh), so the bytes
-// are those of the row-wise quantizer.  Bound by HBM: reads 4 D bytes and
-// writes 2 D (or 4 D) a row.
+// twice the time of the rest).  e4m3: the steps are the quantizer's
+// (quant_common.cuh), so the bytes are those of the row-wise quantizer; K's and
+// V's amax share the words of one shuffle reduction over the row's D / 8 lanes,
+// and each lane then divides for one of the 2 U scales.  Reads 4 D bytes and
+// writes 2 D (or 4 D) a row: HBM bounds it, and the instruction rate is near
+// (254 instructions a thread and row before the sharing, and 71 % of all issue
+// slots).
 template <int D, bool E4M3, bool F16, int U>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs a) {
   constexpr int kLanes = D / 8;                     // threads a row
@@ -35,13 +38,19 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
   const int c = threadIdx.x % kLanes;
   const uint32_t rows = static_cast<uint32_t>(a.tokens) * H, begin = blockIdx.x * kTokens;
   const uint32_t r0 = begin + threadIdx.x / kLanes;
+  const uint32_t next_tok = kAtOnce / H, next_head = kAtOnce % H;
   uint4 k[U], v[U];
   uint32_t tok[U], head[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const uint32_t r = r0 + u * kAtOnce;
-    tok[u] = r / H;
-    head[u] = r - tok[u] * H;
+    tok[u] = u == 0 ? r / H : tok[u - 1] + next_tok;
+    head[u] = u == 0 ? r - tok[u] * H : head[u - 1] + next_head;
+    if (head[u] >= H) {
+      head[u] -= H;
+      ++tok[u];
+    }
+    k[u] = v[u] = make_uint4(0, 0, 0, 0);
     if (r < rows) {
       k[u] = __ldcs(reinterpret_cast<const uint4*>(a.k_new + tok[u] * a.k_tok + head[u] * a.k_head) + c);
       v[u] = __ldcs(reinterpret_cast<const uint4*>(a.v_new + tok[u] * a.v_tok + head[u] * a.v_head) + c);
@@ -84,34 +93,62 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
     offset[i] = off;
   }
   __syncthreads();
+  int64_t off[U];  // of the row; -1: left out
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    if (r0 + u * kAtOnce >= rows) return;  // whole rows: the shuffles below stay in a row
-    const uint32_t i = tok[u] - t0;
-    if (offset[i] < 0) continue;
-    const int64_t off = offset[i] + head[u] * a.kv.s_head;
-    if constexpr (E4M3) {
-      uint32_t mk = quant::absmax8(k[u]), mv = quant::absmax8(v[u]);
-      const unsigned lanes =
-          kLanes == 32 ? 0xffffffffu : ((1u << (kLanes % 32)) - 1) << (threadIdx.x & 31 & ~(kLanes - 1));
+    off[u] = -1;
+    if (r0 + u * kAtOnce < rows && offset[tok[u] - t0] >= 0)
+      off[u] = offset[tok[u] - t0] + static_cast<int64_t>(head[u]) * a.kv.s_head;
+  }
+  if constexpr (E4M3) {
+    uint32_t m[U];  // amax bits: K's in the low half, V's in the high one
 #pragma unroll
-      for (int s = kLanes / 2; s > 0; s /= 2) {
-        mk = max(mk, __shfl_xor_sync(lanes, mk, s));
-        mv = max(mv, __shfl_xor_sync(lanes, mv, s));
-      }
-      const float sk = quant::scale_from_amax_bits<F16>(mk), sv = quant::scale_from_amax_bits<F16>(mv);
-      reinterpret_cast<uint2*>(a.kv.k + off)[c] = quant::quant8_any<F16>(k[u], __frcp_rn(sk), isfinite(sk));
-      reinterpret_cast<uint2*>(a.kv.v + off)[c] = quant::quant8_any<F16>(v[u], __frcp_rn(sv), isfinite(sv));
-      if (c == 0) {
-        const int64_t at = scale_at[i] + static_cast<int64_t>(head[u]) * a.kv.page_size;
-        a.kv.ks[at] = sk;
-        a.kv.vs[at] = sv;
-      }
-    } else {
-      reinterpret_cast<uint4*>(a.kv.k + 2 * off)[c] = k[u];
-      reinterpret_cast<uint4*>(a.kv.v + 2 * off)[c] = v[u];
+    for (int u = 0; u < U; ++u) {
+      m[u] = quant::absmax8(k[u]) | quant::absmax8(v[u]) << 16;
+#pragma unroll
+      for (int x = kLanes / 2; x > 0; x /= 2) m[u] = __vmaxu2(m[u], __shfl_xor_sync(0xffffffffu, m[u], x));
     }
-    if (a.weights.w && c == 0) a.weights.w[weight_at[i] + head[u] * a.weights.s_head] = 0.f;
+    constexpr int kRounds = (2 * U + kLanes - 1) / kLanes;
+    float mul[kRounds];  // of scale j = c + round * kLanes: row j / 2, K or V
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+      const int j = c + i * kLanes;
+      uint32_t mine = m[0], at_tok = tok[0], at_head = head[0];
+      bool store = off[0] >= 0;
+#pragma unroll
+      for (int u = 1; u < U; ++u)
+        if (j / 2 == u) {
+          mine = m[u];
+          at_tok = tok[u];
+          at_head = head[u];
+          store = off[u] >= 0;
+        }
+      const float scale = quant::scale_from_amax_bits<F16>(j % 2 ? mine >> 16 : mine & 0xffffu);
+      mul[i] = __frcp_rn(scale);
+      if (j < 2 * U && store)
+        (j % 2 ? a.kv.vs : a.kv.ks)[scale_at[at_tok - t0] + static_cast<int64_t>(at_head) * a.kv.page_size] = scale;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float qk = __shfl_sync(0xffffffffu, mul[2 * u / kLanes], 2 * u % kLanes, kLanes);
+      const float qv = __shfl_sync(0xffffffffu, mul[(2 * u + 1) / kLanes], (2 * u + 1) % kLanes, kLanes);
+      if (off[u] < 0) continue;
+      // a scale that is inf or NaN has a reciprocal that is not positive
+      reinterpret_cast<uint2*>(a.kv.k + off[u])[c] = quant::quant8_any<F16>(k[u], qk, qk > 0.f);
+      reinterpret_cast<uint2*>(a.kv.v + off[u])[c] = quant::quant8_any<F16>(v[u], qv, qv > 0.f);
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (off[u] < 0) continue;
+      reinterpret_cast<uint4*>(a.kv.k + 2 * off[u])[c] = k[u];
+      reinterpret_cast<uint4*>(a.kv.v + 2 * off[u])[c] = v[u];
+    }
+  }
+  if (a.weights.w && c == 0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (off[u] >= 0) a.weights.w[weight_at[tok[u] - t0] + head[u] * a.weights.s_head] = 0.f;
   }
 }
 
@@ -128,11 +165,12 @@ cudaError_t append_u(const AppendArgs& a, cudaStream_t st) {
   return cudaGetLastError();
 }
 
-// Four rows a thread once the GPU is full all the same (148 SMs of 2048 threads).
+// Two rows a thread once the GPU is full all the same (148 SMs of 2048 threads): 48 prompts of 8
+// heads took 172 us with one row, 139 with two, 145 with four, 192 with eight.
 template <int D>
 cudaError_t append_d(const AppendArgs& a, cudaStream_t st) {
   const int64_t threads = static_cast<int64_t>(a.tokens) * a.kv.heads * (D / 8);
-  return threads >= 4LL * 148 * 2048 ? append_u<D, 4>(a, st) : append_u<D, 1>(a, st);
+  return threads >= 2LL * 148 * 2048 ? append_u<D, 2>(a, st) : append_u<D, 1>(a, st);
 }
 
 // Weights order: a key is larger when the weight is; -0 equals 0 and any NaN
