@@ -158,6 +158,8 @@ int rp_paged_decode(const rp_paged_kv* kv, const void* q, const int64_t* q_strid
     return set_last_error(RP_ERR_INVALID, "the query and a 16-bit cache must share a dtype");
   if (Hq <= 0 || Hq % a.kv.heads != 0)
     return set_last_error(RP_ERR_INVALID, "%d query heads are no multiple of %d KV heads", Hq, a.kv.heads);
+  if (rp::pool_unit(a.kv) == 0)
+    return set_last_error(RP_ERR_UNSUPPORTED, "the pool's strides address more than 2^32 units of their common power of two");
   if (Hq > 65535) return set_last_error(RP_ERR_UNSUPPORTED, "more than 65535 query heads");
   if (!std::isfinite(sm_scale)) return set_last_error(RP_ERR_INVALID, "sm_scale is not finite");
   if (B == 0) return RP_OK;

@@ -109,6 +109,25 @@ struct ScoreArgs {
 };
 cudaError_t launch_token_logprobs(const ScoreArgs& a, cudaStream_t st);
 
+// Bytes of which every stride of the pool is a multiple (a power of two), if a
+// row's offset then fits 32 bits; else 0.  A contiguous pool's unit is a row or
+// more, so that only pools of terabytes, or of odd strides and over 64 GB, have
+// none.
+inline int64_t pool_unit(const PagedPool& kv) {
+  const int64_t size = kv.dtype == kKvE4m3 ? 1 : 2, all = (kv.s_page | kv.s_head | kv.s_slot) * size;
+  const int64_t unit = all == 0 ? 16 : all & -all;
+  const int64_t rows[3] = {kv.num_pages - 1, kv.heads - 1, kv.page_size - 1};
+  const int64_t strides[3] = {kv.s_page, kv.s_head, kv.s_slot};
+  uint64_t span = 0;  // in units
+  for (int i = 0; i < 3; ++i) {
+    const uint64_t n = static_cast<uint64_t>(strides[i] * size / unit);
+    if (rows[i] == 0) continue;
+    if (n > 0xFFFFFFFFu) return 0;
+    span += n * static_cast<uint64_t>(rows[i]);
+  }
+  return span > 0xFFFFFFFFu || unit > 0x80000000LL ? 0 : unit;
+}
+
 // Per-device settings of the launchers are kept for this many devices.
 constexpr int kMaxDevices = 64;
 inline int current_device() {

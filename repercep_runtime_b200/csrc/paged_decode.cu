@@ -58,15 +58,17 @@ struct Cfg {
   static constexpr bool kBf16 = KV == kKvBf16;
   static constexpr int kRow = D * (kFp8 ? 1 : 2);   // bytes of a row
   static constexpr int kChunks = kRow / 16;         // 16-byte chunks of a row
-  static constexpr int kKeys = kRow >= 256 ? 16 : 32;  // keys of a warp's step
+  static constexpr int kFrags = D / 16 * NT;  // accumulator fragments (float4 a lane)
+  // keys of a warp's step: 16 where that makes 8 KB (a stage holds a warp's accumulators at times)
+  static constexpr int kKeys = 32 * kRow >= 8192 && 32 * kRow >= kFrags * 512 ? 16 : 32;
   static constexpr int kTile = kKeys * kWarps;
   static constexpr int kRowsBytes = kKeys * kRow;
   static constexpr int kStage = 2 * kRowsBytes + (kFp8 ? kKeys * 8 : 0);
-  // about 24 KB in flight a warp, two CTAs an SM
-  static constexpr int kStages = 2 * kRowsBytes >= 8192 ? 3 : 2 * kRowsBytes >= 4096 ? 6 : 8;
-  static constexpr int kFrags = D / 16 * NT;  // accumulator fragments (float4 a lane)
+  static_assert(kStage >= kFrags * 512, "a stage holds a warp's accumulators");
+  // 16 KB a warp, so that three CTAs share an SM
+  static constexpr int kStages = 2 * kRowsBytes >= 8192 ? 2 : 2 * kRowsBytes >= 4096 ? 4 : 6;
   static constexpr int kRing = kStages * kStage;
-  static constexpr int kSmem = kWarps * kRing + 2 * kFrags * 512 + kWarps * NT * 8 * 8 + kWarps * kStages * 4;
+  static constexpr int kSmem = kWarps * kRing + kWarps * NT * 8 * 8 + kWarps * kStages * 4;
 };
 
 // What a CTA left for the join: the item it began (tile 0) without ending it
@@ -80,6 +82,9 @@ struct Params {
   int G;       // query heads of a KV head
   int groups;  // column groups of a KV head (NT * 8 query heads each)
   int shift;   // log2 of the page size, or -1
+  // The pool's strides in units of their largest common power of two (bytes):
+  // a row's offset is then a 32-bit number.
+  uint32_t u_page, u_head, u_slot, unit;
   int grid;    // CTAs of the main kernel
   int score_pitch;
   float4* part_o;  // (grid * 2, kFrags, 32)
@@ -164,6 +169,11 @@ __device__ __forceinline__ uint16_t round16(float x, bool f16) {
 }
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
 
+// Programmatic launches: what follows may be launched; what came before is
+// complete and its memory visible.
+__device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // A place in the line of tiles: sequence, item of the sequence (KV head and
 // column group), tile of the item.
 struct Place {
@@ -211,13 +221,13 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int row = lane >> 2, pair = lane & 3;
   const uint32_t ring = smem_u32(smem) + warp * C::kRing;
-  float4* join = reinterpret_cast<float4*>(smem + kWarps * C::kRing);
-  float* sm_m = reinterpret_cast<float*>(smem + kWarps * C::kRing + 2 * C::kFrags * 512);
+  float* sm_m = reinterpret_cast<float*>(smem + kWarps * C::kRing);
   float* sm_l = sm_m + kWarps * NT * 8;
   uint32_t* live = reinterpret_cast<uint32_t*>(sm_l + kWarps * NT * 8) + warp * S;
   const PagedPool& kv = p.a.kv;
   const int items = kv.heads * p.groups, B = p.a.t.B;
 
+  launch_next();
   // ---- this CTA's run of tiles: a prefix sum over the sequences
   __shared__ long long sums[kWarps];
   __shared__ Place at;
@@ -275,7 +285,9 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
   int to_load = static_cast<int>(last - first), left = to_load;
 
   // ---- loads: lane's key of the warp's slice, its page id one step ahead
-  const int my_key = lane % C::kKeys;
+  const int my_key = lane % C::kKeys, my_col = lane % C::kChunks;
+  const uint8_t* k_col = kv.k + my_col * 16;
+  const uint8_t* v_col = kv.v + my_col * 16;
   int page = 0;
   const auto fetch_page = [&] {
     const int key = load.tile * C::kTile + warp * C::kKeys + my_key;
@@ -297,11 +309,10 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
       }
       const uint32_t mask = __ballot_sync(0xffffffffu, ok);
       if (lane == 0) live[stage] = mask;
-      int64_t off = 0;
+      uint32_t off = 0;
       if (ok) {
-        const int slot = p.shift >= 0 ? key & (kv.page_size - 1) : key % kv.page_size;
-        off = page * kv.s_page + head * kv.s_head + slot * kv.s_slot;
-        if constexpr (!C::kFp8) off *= 2;
+        const uint32_t slot = p.shift >= 0 ? key & (kv.page_size - 1) : key % kv.page_size;
+        off = page * p.u_page + head * p.u_head + slot * p.u_slot;
         if constexpr (C::kFp8) {
           const int64_t i = (static_cast<int64_t>(page) * kv.heads + head) * kv.page_size + slot;
           if (lane < C::kKeys) {
@@ -318,14 +329,14 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
       if (key - my_key < load.n) {  // some of the slice is in the sequence: the rest of it is zeroed
 #pragma unroll
         for (int i = 0; i < C::kKeys * C::kChunks / 32; ++i) {
-          const int c = i * 32 + lane, r = c / C::kChunks, col = c % C::kChunks;
-          const int64_t o = __shfl_sync(0xffffffffu, off, r);
+          const int r = i * (32 / C::kChunks) + lane / C::kChunks;
+          const uint64_t o = static_cast<uint64_t>(__shfl_sync(0xffffffffu, off, r)) * p.unit;
           const bool read = (mask >> r) & 1;
           constexpr int kRsh = C::kRow >= 128 ? 0 : C::kRow == 64 ? 1 : 2;
           constexpr int kMask = C::kChunks >= 8 ? 7 : C::kChunks - 1;
-          const uint32_t dst = base + r * C::kRow + ((col ^ ((r >> kRsh) & kMask)) << 4);
-          cp_async16(dst, kv.k + o + col * 16, read);
-          cp_async16(dst + C::kRowsBytes, kv.v + o + col * 16, read);
+          const uint32_t dst = base + r * C::kRow + ((my_col ^ ((r >> kRsh) & kMask)) << 4);
+          cp_async16(dst, k_col + o, read);
+          cp_async16(dst + C::kRowsBytes, v_col + o, read);
         }
       }
       --to_load;
@@ -628,31 +639,39 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
           o[dt][nt][2 + j] *= f;
         }
       }
-    const auto put = [&](int buf) {
+    // through the stage that each warp read last: its next load goes there, after the barriers
+    const int idle_stage = stage == 0 ? S - 1 : stage - 1;
+    const auto buffer = [&](int w) {
+      return reinterpret_cast<float4*>(smem + w * C::kRing + idle_stage * C::kStage) + lane;
+    };
+    const auto put = [&] {
+      float4* dst = buffer(warp);
 #pragma unroll
       for (int i = 0; i < C::kFrags; ++i) {
         const float(&c)[4] = o[i / NT][i % NT];
-        join[(buf * C::kFrags + i) * 32 + lane] = make_float4(c[0], c[1], c[2], c[3]);
+        dst[i * 32] = make_float4(c[0], c[1], c[2], c[3]);
       }
     };
-    const auto take = [&](int buf) {
+    const auto take = [&](int w) {
+      const float4* src = buffer(w);
 #pragma unroll
       for (int i = 0; i < C::kFrags; ++i) {
         float(&c)[4] = o[i / NT][i % NT];
-        const float4 y = join[(buf * C::kFrags + i) * 32 + lane];
+        const float4 y = src[i * 32];
         c[0] += y.x;
         c[1] += y.y;
         c[2] += y.z;
         c[3] += y.w;
       }
     };
-    if (warp >= 2) put(warp - 2);
+    if (warp >= 2) put();
     __syncthreads();
-    if (warp < 2) take(warp);
-    if (warp == 1) put(1);
+    if (warp < 2) take(warp + 2);
+    if (warp == 1) put();
+    __syncthreads();
+    if (warp == 0) take(1);
     __syncthreads();
     if (warp == 0) {
-      take(1);
       if (begins && ends) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -712,6 +731,8 @@ __global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const Params 
   __shared__ float4 sums[kJoinThreads];
   __shared__ float sm_inv[NT * 8];
   __shared__ int count;
+  launch_next();
+  wait_previous();
   const Cut cut = p.cuts[blockIdx.x];
   if (cut.begun < 0) return;
   const int item = cut.begun, first_slot = blockIdx.x * 2 + cut.begun_slot;
@@ -784,23 +805,64 @@ __global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const Params 
   }
 }
 
-// Every key's weights, summed over the query heads of its KV head in order.
+// Every key's weights, summed over the query heads of its KV head in order;
+// four keys a thread.
 __global__ void __launch_bounds__(256) decode_weights_kernel(const Params p) {
+  wait_previous();
   const int h = blockIdx.y, b = blockIdx.z;
   const int n = table_length(p.a.t, p.a.kv.page_size, b, p.a.status);
   const int64_t row = static_cast<int64_t>(b) * p.a.Hq + h * p.G;
   const float* scores = p.scores + row * p.score_pitch;
   const float* lse2 = p.lse2 + row;
   float* dst = p.a.weights.w + b * p.a.weights.s_seq + h * p.a.weights.s_head;
-  for (int j = blockIdx.x * 256 + threadIdx.x; j < n; j += gridDim.x * 256) {
-    float w = 0.f;
+  const bool whole = (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
+  for (int j = (blockIdx.x * 256 + threadIdx.x) * 4; j < n; j += gridDim.x * 1024) {
+    float w[4] = {0.f, 0.f, 0.f, 0.f}, old[4];
+    const bool four = whole && j + 4 <= n;
+    if (four) {
+      const float4 y = *reinterpret_cast<const float4*>(dst + j);
+      old[0] = y.x;
+      old[1] = y.y;
+      old[2] = y.z;
+      old[3] = y.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) old[i] = j + i < n ? dst[j + i] : 0.f;
+    }
 #pragma unroll 4
     for (int g = 0; g < p.G; ++g) {
-      const float y = __ldg(lse2 + g);
-      w += ex2(__ldg(scores + static_cast<int64_t>(g) * p.score_pitch + j) - finite_or_zero(y));
+      const float y = finite_or_zero(__ldcg(lse2 + g));
+      // the rows of scores are whole 16-byte vectors; what lies past n is not used
+      const float4 x = __ldcs(reinterpret_cast<const float4*>(scores + static_cast<int64_t>(g) * p.score_pitch + j));
+      w[0] += ex2(x.x - y);
+      w[1] += ex2(x.y - y);
+      w[2] += ex2(x.z - y);
+      w[3] += ex2(x.w - y);
     }
-    dst[j] += w;
+    if (four) {
+      *reinterpret_cast<float4*>(dst + j) = make_float4(old[0] + w[0], old[1] + w[1], old[2] + w[2], old[3] + w[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (j + i < n) dst[j + i] = old[i] + w[i];
+    }
   }
+}
+
+// A launch that may begin while the launch before it ends (it waits for it).
+template <typename F, typename A>
+cudaError_t launch_after(F* kernel, dim3 grid, int threads, size_t smem, cudaStream_t st, const A& arg) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, arg);
 }
 
 int sm_count(int dev) {
@@ -859,8 +921,8 @@ cudaError_t launch(Params p, cudaStream_t st) {
   decode_kernel<KV, D, NT><<<p.grid, kThreads, C::kSmem, st>>>(p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  decode_join_kernel<KV, D, NT><<<p.grid, kJoinThreads, p.grid * NT * 8 * 4, st>>>(p);
-  return cudaGetLastError();
+  return launch_after(decode_join_kernel<KV, D, NT>, dim3(p.grid), kJoinThreads,
+                      static_cast<size_t>(p.grid) * NT * 8 * 4, st, p);
 }
 
 template <int KV, int D>
@@ -897,6 +959,13 @@ cudaError_t launch_paged_decode(const PagedDecodeArgs& a, cudaStream_t st) {
   p.shift = -1;
   for (int s = 0; s < 31; ++s)
     if (a.kv.page_size == 1 << s) p.shift = s;
+  const int size = a.kv.dtype == kKvE4m3 ? 1 : 2;
+  const int64_t unit = pool_unit(a.kv);
+  if (unit == 0) return cudaErrorInvalidValue;
+  p.u_page = static_cast<uint32_t>(a.kv.s_page * size / unit);
+  p.u_head = static_cast<uint32_t>(a.kv.s_head * size / unit);
+  p.u_slot = static_cast<uint32_t>(a.kv.s_slot * size / unit);
+  p.unit = static_cast<uint32_t>(unit);
   p.score_pitch = ws.pitch;
   p.part_o = reinterpret_cast<float4*>(base);
   p.part_ml = reinterpret_cast<float*>(base + ws.part_ml);
@@ -911,10 +980,10 @@ cudaError_t launch_paged_decode(const PagedDecodeArgs& a, cudaStream_t st) {
   }
   const int cap = a.t.pages * a.kv.page_size;
   if (e != cudaSuccess || !weights || cap == 0) return e;
-  // enough CTAs for the SMs, at most one per 256 positions
-  const int rows = a.kv.heads * a.t.B, want = (16 * sm_count(current_device()) + rows - 1) / rows, most = (cap + 255) / 256;
-  decode_weights_kernel<<<dim3(want < most ? want : most, a.kv.heads, a.t.B), 256, 0, st>>>(p);
-  return cudaGetLastError();
+  // enough CTAs for the SMs, at most one per 1024 positions
+  const int rows = a.kv.heads * a.t.B, most = (cap + 1023) / 1024;
+  const int want = (16 * sm_count(current_device()) + rows - 1) / rows;
+  return launch_after(decode_weights_kernel, dim3(want < most ? want : most, a.kv.heads, a.t.B), 256, 0, st, p);
 }
 
 }  // namespace rp
