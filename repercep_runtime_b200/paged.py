@@ -26,8 +26,10 @@ raises).
 
 from __future__ import annotations
 
-from ctypes import byref
+import functools
+from ctypes import byref, c_int64
 from dataclasses import dataclass, field
+from typing import NamedTuple
 
 import torch
 
@@ -37,6 +39,8 @@ FP8 = torch.float8_e4m3fn
 HEAD_DIMS = (32, 64, 128, 256)
 _HALF = {torch.bfloat16: _lib.RP_DTYPE_BF16, torch.float16: _lib.RP_DTYPE_F16}
 _KV = {torch.bfloat16: _lib.RP_KV_BF16, torch.float16: _lib.RP_KV_F16, FP8: _lib.RP_KV_E4M3}
+_I64x2 = c_int64 * 2
+_I64x4 = c_int64 * 4
 
 
 @dataclass(frozen=True, eq=False)
@@ -56,6 +60,8 @@ class PagedKV:
     heads: int = field(init=False)
     page_size: int = field(init=False)
     head_dim: int = field(init=False)
+    dtype: torch.dtype = field(init=False)
+    device: torch.device = field(init=False)
 
     def __post_init__(self) -> None:
         k, v = self.k, self.v
@@ -85,24 +91,17 @@ class PagedKV:
                 raise ValueError(f"{name} must be contiguous fp32 ({pages}, {heads}, {size}) on {k.device}")
         for name, value in (("num_pages", pages), ("heads", heads), ("page_size", size), ("head_dim", D)):
             object.__setattr__(self, name, int(value))
-
-    @property
-    def dtype(self) -> torch.dtype:
-        return self.k.dtype
-
-    @property
-    def device(self) -> torch.device:
-        return self.k.device
+        object.__setattr__(self, "dtype", k.dtype)
+        object.__setattr__(self, "device", k.device)
+        s = k.stride()
+        strides = s[:3] if bhsd else (s[0], s[2], s[1])
+        object.__setattr__(self, "_geometry", (strides, _KV[k.dtype], self.num_pages, self.heads, self.page_size, D))
 
     def _struct(self) -> _lib.PagedKVStruct:
-        k = self.k
-        s = k.stride()
-        strides = s[:3] if self.layout == "bhsd" else (s[0], s[2], s[1])
         ks, vs = self.k_scales, self.v_scales
         return _lib.PagedKVStruct(
-            k.data_ptr(), self.v.data_ptr(),
-            ks.data_ptr() if ks is not None else None, vs.data_ptr() if vs is not None else None,
-            strides, _KV[k.dtype], self.num_pages, self.heads, self.page_size, self.head_dim,
+            self.k.data_ptr(), self.v.data_ptr(),
+            None if ks is None else ks.data_ptr(), None if vs is None else vs.data_ptr(), *self._geometry,
         )  # fmt: skip
 
 
@@ -124,53 +123,46 @@ def alloc(
     return PagedKV(k, v, scales[0], scales[1], layout)
 
 
-def _stream(device: torch.device) -> int:
-    return int(torch.cuda.current_stream(device).cuda_stream)
-
-
-def _on(device: torch.device):  # type: ignore[no-untyped-def]
-    """The library launches on the current device: make it ``device``."""
-    return torch.cuda.device(device)
-
-
 def _int32(x: torch.Tensor, name: str, shape: tuple[int, ...], device: torch.device) -> None:
-    if x.dtype != torch.int32 or x.device != device or tuple(x.shape) != shape:
+    if x.dtype != torch.int32 or x.device != device or x.shape != shape:
         raise ValueError(f"{name} must be int32 {shape} on {device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
 
 
-def _table(cache: PagedKV, page_table: torch.Tensor, lengths: torch.Tensor) -> tuple[int, int]:
-    """Checks a page table and its lengths; (sequences, pages a row)."""
-    if page_table.dim() != 2:
-        raise ValueError("page_table must be 2-D (sequences, pages)")
-    B, pages = page_table.shape
-    _int32(page_table, "page_table", (B, pages), cache.device)
-    _int32(lengths, "lengths", (B,), cache.device)
-    if pages > 1 and page_table.stride(1) != 1:
-        raise ValueError("page_table rows must be contiguous")
+def _table(device: torch.device, name: str, table: torch.Tensor, B: int | None = None) -> tuple[int, int, int]:
+    """Checks a page table; (sequences, pages a row, row stride)."""
+    if table.dim() != 2:
+        raise ValueError(f"{name} must be 2-D (sequences, pages)")
+    rows, pages = table.shape
+    _int32(table, name, (rows if B is None else B, pages), device)
+    stride, step = table.stride()
+    if pages > 1 and step != 1:
+        raise ValueError(f"{name} rows must be contiguous")
+    return rows, pages, stride if rows > 1 else pages
+
+
+def _lengths(device: torch.device, lengths: torch.Tensor, B: int) -> None:
+    _int32(lengths, "lengths", (B,), device)
     if B > 1 and lengths.stride(0) != 1:
         raise ValueError("lengths must be contiguous")
-    return B, pages
-
-
-def _row_stride(table: torch.Tensor) -> int:
-    B, pages = table.shape
-    return table.stride(0) if B > 1 else pages
 
 
 def _weights(cache: PagedKV, w: torch.Tensor | None, B: int, pages: int):  # type: ignore[no-untyped-def]
     """(pointer, strides, columns) of accumulated weights."""
     if w is None:
         return None, None, 0
-    if w.dtype != torch.float32 or w.device != cache.device or w.dim() != 3 or tuple(w.shape[:2]) != (B, cache.heads):
+    if w.dim() != 3 or w.dtype != torch.float32 or w.device != cache.device:
         raise ValueError(f"weights must be fp32 ({B}, {cache.heads}, positions) on {cache.device}")
-    cols = w.shape[2]
+    rows, heads, cols = w.shape
+    if rows != B or heads != cache.heads:
+        raise ValueError(f"weights must be fp32 ({B}, {cache.heads}, positions) on {cache.device}")
     if cols < pages * cache.page_size:
         raise ValueError(f"weights hold {cols} positions, the page table {pages * cache.page_size}")
-    if cols > 1 and w.stride(2) != 1:
+    s0, s1, s2 = w.stride()
+    if cols > 1 and s2 != 1:
         raise ValueError("weights must have unit-stride positions")
-    if (B > 1 and w.stride(0) == 0) or (cache.heads > 1 and w.stride(1) == 0):
+    if (B > 1 and s0 == 0) or (heads > 1 and s1 == 0):
         raise ValueError("weights of sequences or heads overlap")
-    return w.data_ptr(), _lib.i64_array((w.stride(0), w.stride(1))), cols
+    return w.data_ptr(), _I64x2(s0, s1), cols
 
 
 def append(
@@ -191,36 +183,43 @@ def append(
     every sequence gets one token.  An e4m3 cache takes each row's scale and
     bytes from ``linear.quantize_rows``'s recipe.  ``weights`` are zeroed at
     the new positions."""
-    B, pages = _table(cache, page_table, lengths)
-    dtype = k_new.dtype
-    if k_new.dim() != 3 or k_new.shape != v_new.shape or tuple(k_new.shape[1:]) != (cache.heads, cache.head_dim):
+    device, dtype = cache.device, k_new.dtype
+    B, pages, row = _table(device, "page_table", page_table)
+    _lengths(device, lengths, B)
+    if k_new.dim() != 3 or k_new.shape != v_new.shape or k_new.shape[1:] != (cache.heads, cache.head_dim):
         raise ValueError(f"k_new and v_new must be (tokens, {cache.heads}, {cache.head_dim})")
     if dtype not in _HALF or v_new.dtype != dtype or (cache.dtype != FP8 and dtype != cache.dtype):
         raise ValueError(f"k_new and v_new must be {'bf16 or fp16' if cache.dtype == FP8 else cache.dtype}, got {dtype}")
-    if k_new.device != cache.device or v_new.device != cache.device:
-        raise ValueError(f"k_new and v_new must be on {cache.device}")
-    if k_new.stride(2) != 1 or v_new.stride(2) != 1:
+    if k_new.device != device or v_new.device != device:
+        raise ValueError(f"k_new and v_new must be on {device}")
+    (k0, k1, k2), (v0, v1, v2) = k_new.stride(), v_new.stride()
+    if k2 != 1 or v2 != 1:
         raise ValueError("k_new and v_new must have a unit-stride head dim")
     tokens = k_new.shape[0]
     if starts is not None:
-        _int32(starts, "starts", (B + 1,), cache.device)
+        _int32(starts, "starts", (B + 1,), device)
         if starts.stride(0) != 1:
             raise ValueError("starts must be contiguous")
     elif tokens != B:
         raise ValueError(f"{tokens} new tokens for {B} sequences need starts")
     w, w_strides, w_cols = _weights(cache, weights, B, pages)
     out = torch.empty_like(lengths)
-    lib = _lib.load()
-    with _on(cache.device):
-        rc = lib.rp_paged_append(
-            byref(cache._struct()), k_new.data_ptr(), v_new.data_ptr(),
-            _lib.i64_array((k_new.stride(0), k_new.stride(1), v_new.stride(0), v_new.stride(1))),
-            _HALF[dtype], tokens, starts.data_ptr() if starts is not None else None,
-            page_table.data_ptr(), _row_stride(page_table), pages, lengths.data_ptr(), B,
-            w, w_strides, w_cols, out.data_ptr(), _stream(cache.device),
-        )  # fmt: skip
-    _lib.check("rp_paged_append", rc)
+    _lib.launch(
+        device.index, "rp_paged_append", byref(cache._struct()), k_new.data_ptr(), v_new.data_ptr(),
+        _I64x4(k0, k1, v0, v1), _HALF[dtype], tokens, None if starts is None else starts.data_ptr(),
+        page_table.data_ptr(), row, pages, lengths.data_ptr(), B, w, w_strides, w_cols, out.data_ptr(),
+    )  # fmt: skip
     return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _decode_workspace(geometry: tuple, B: int, Hq: int, pages: int, with_weights: bool) -> int:
+    """``rp_paged_decode_workspace_bytes`` of a pool's geometry."""
+    need = _lib._c_size_t(0)
+    kv = _lib.PagedKVStruct(None, None, None, None, *geometry)
+    rc = _lib.load().rp_paged_decode_workspace_bytes(byref(kv), B, Hq, pages, int(with_weights), byref(need))
+    _lib.check("rp_paged_decode_workspace_bytes", rc)
+    return int(need.value)
 
 
 def decode(
@@ -244,49 +243,45 @@ def decode(
     zeros and -inf.  ``weights`` fp32 (sequences, heads, positions): every
     key's attention weight, summed over the query heads of its KV head, is
     added in place."""
-    B, pages = _table(cache, page_table, lengths)
-    if q.dim() != 3 or q.shape[0] != B or q.shape[2] != cache.head_dim:
-        raise ValueError(f"q must be ({B}, query heads, {cache.head_dim}), got {tuple(q.shape)}")
-    Hq = q.shape[1]
+    device, dtype = cache.device, q.dtype
+    B, pages, row = _table(device, "page_table", page_table)
+    _lengths(device, lengths, B)
+    shape = q.shape
+    if len(shape) != 3 or shape[0] != B or shape[2] != cache.head_dim:
+        raise ValueError(f"q must be ({B}, query heads, {cache.head_dim}), got {tuple(shape)}")
+    Hq = shape[1]
     if Hq == 0 or Hq % cache.heads != 0:
         raise ValueError(f"{Hq} query heads are no multiple of {cache.heads} KV heads")
-    if q.dtype not in _HALF or (cache.dtype != FP8 and q.dtype != cache.dtype):
-        raise ValueError(f"q must be {'bf16 or fp16' if cache.dtype == FP8 else cache.dtype}, got {q.dtype}")
-    if q.device != cache.device:
-        raise ValueError(f"q must be on {cache.device}")
-    if q.stride(2) != 1:
+    if dtype not in _HALF or (cache.dtype != FP8 and dtype != cache.dtype):
+        raise ValueError(f"q must be {'bf16 or fp16' if cache.dtype == FP8 else cache.dtype}, got {dtype}")
+    if q.device != device:
+        raise ValueError(f"q must be on {device}")
+    q0, q1, q2 = q.stride()
+    if q2 != 1:
         raise ValueError("q must have a unit-stride head dim")
     if scale is not None and not 0.0 < scale < float("inf"):
         raise ValueError(f"scale must be positive and finite, got {scale}")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(2) != 1:
+        out = q.new_empty(shape)
+    elif out.shape != shape or out.dtype != dtype or out.device != device or out.stride(2) != 1:
         raise ValueError("out must have q's shape, dtype and device, with a unit-stride head dim")
-    if (B > 1 and out.stride(0) == 0) or (Hq > 1 and out.stride(1) == 0):
+    o0, o1, _ = out.stride()
+    if (B > 1 and o0 == 0) or (Hq > 1 and o1 == 0):
         raise ValueError("rows of out overlap")
-    lse = torch.empty((B, Hq), dtype=torch.float32, device=q.device) if return_lse else None
+    lse = torch.empty((B, Hq), dtype=torch.float32, device=device) if return_lse else None
     w, w_strides, w_cols = _weights(cache, weights, B, pages)
-    lib = _lib.load()
-    kv = byref(cache._struct())
-    need = _lib._c_size_t(0)
-    rc = lib.rp_paged_decode_workspace_bytes(kv, B, Hq, pages, 1 if weights is not None else 0, byref(need))
-    _lib.check("rp_paged_decode_workspace_bytes", rc)
-    ws = torch.empty(need.value, dtype=torch.uint8, device=q.device)
-    with _on(cache.device):
-        rc = lib.rp_paged_decode(
-            kv, q.data_ptr(), _lib.i64_array((q.stride(0), q.stride(1))), _HALF[q.dtype], B, Hq,
-            page_table.data_ptr(), _row_stride(page_table), pages, lengths.data_ptr(),
-            float(scale) if scale is not None else 0.0,
-            out.data_ptr(), _lib.i64_array((out.stride(0), out.stride(1))),
-            lse.data_ptr() if lse is not None else None, w, w_strides, w_cols,
-            ws.data_ptr(), need.value, _stream(cache.device),
-        )  # fmt: skip
-    _lib.check("rp_paged_decode", rc)
+    need = _decode_workspace(cache._geometry, B, Hq, pages, weights is not None)
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    _lib.launch(
+        device.index, "rp_paged_decode", byref(cache._struct()), q.data_ptr(), _I64x2(q0, q1), _HALF[dtype], B, Hq,
+        page_table.data_ptr(), row, pages, lengths.data_ptr(), 0.0 if scale is None else scale,
+        out.data_ptr(), _I64x2(o0, o1), None if lse is None else lse.data_ptr(), w, w_strides, w_cols,
+        ws.data_ptr(), need,
+    )  # fmt: skip
     return (out, lse) if return_lse else out
 
 
-@dataclass(frozen=True, eq=False)
-class Evicted:
+class Evicted(NamedTuple):
     """``kept`` (sequences, heads, budget) int32 old positions in order, -1 past
     the end; ``lengths`` (sequences,) after the cut; ``weights`` (sequences,
     heads, positions of the new table) of the kept tokens, 0 past the end."""
@@ -314,13 +309,10 @@ def evict(
     positions 0, 1, ... of ``out_table`` (sequences, pages), whose pages must
     be none of ``page_table``'s: nothing is written to those, which other
     sequences may share."""
-    B, pages = _table(cache, page_table, lengths)
-    if out_table.dim() != 2:
-        raise ValueError("out_table must be 2-D (sequences, pages)")
-    out_pages = out_table.shape[1]
-    _int32(out_table, "out_table", (B, out_pages), cache.device)
-    if out_pages > 1 and out_table.stride(1) != 1:
-        raise ValueError("out_table rows must be contiguous")
+    device = cache.device
+    B, pages, row = _table(device, "page_table", page_table)
+    _lengths(device, lengths, B)
+    _, out_pages, out_row = _table(device, "out_table", out_table, B)
     budget, recent = int(budget), int(recent)
     if budget <= 0 or not 0 <= recent <= budget:
         raise ValueError(f"budget must be positive and recent in [0, budget], got {budget} and {recent}")
@@ -329,18 +321,14 @@ def evict(
     if weights is None:
         raise ValueError("evict needs the accumulated weights")
     w, w_strides, w_cols = _weights(cache, weights, B, pages)
-    dev = cache.device
-    kept = torch.empty((B, cache.heads, budget), dtype=torch.int32, device=dev)
+    kept = torch.empty((B, cache.heads, budget), dtype=torch.int32, device=device)
     new_lengths = torch.empty_like(lengths)
-    new_weights = torch.empty((B, cache.heads, out_pages * cache.page_size), dtype=torch.float32, device=dev)
-    lib = _lib.load()
-    with _on(dev):
-        rc = lib.rp_paged_evict(
-            byref(cache._struct()), page_table.data_ptr(), _row_stride(page_table), pages, lengths.data_ptr(), B,
-            w, w_strides, w_cols, out_table.data_ptr(), _row_stride(out_table), out_pages, budget, recent,
-            kept.data_ptr(), new_lengths.data_ptr(), new_weights.data_ptr(), _stream(dev),
-        )  # fmt: skip
-    _lib.check("rp_paged_evict", rc)
+    new_weights = torch.empty((B, cache.heads, out_pages * cache.page_size), dtype=torch.float32, device=device)
+    _lib.launch(
+        device.index, "rp_paged_evict", byref(cache._struct()), page_table.data_ptr(), row, pages, lengths.data_ptr(), B,
+        w, w_strides, w_cols, out_table.data_ptr(), out_row, out_pages, budget, recent,
+        kept.data_ptr(), new_lengths.data_ptr(), new_weights.data_ptr(),
+    )  # fmt: skip
     return Evicted(kept, new_lengths, new_weights)
 
 

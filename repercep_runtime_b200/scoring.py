@@ -12,7 +12,7 @@ runs in the library, which has no fallback (a missing library raises).
 
 from __future__ import annotations
 
-from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
@@ -26,8 +26,7 @@ _LOGITS = {
 }
 
 
-@dataclass(frozen=True, eq=False)
-class TokenScores:
+class TokenScores(NamedTuple):
     """Per row: ``logprobs`` and ``entropy`` fp32 (rows,), ``top_logprobs`` fp32
     and ``top_ids`` int64 (rows, top), largest first, ties to the lowest id."""
 
@@ -54,25 +53,23 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
         raise ValueError("logits have an empty vocabulary")
     if vocab > 1 and logits.stride(1) != 1:
         raise ValueError("logits must have a unit-stride vocabulary")
-    dev = logits.device
-    if tokens.dtype != torch.int64 or tuple(tokens.shape) != (rows,) or tokens.device != dev:
-        raise ValueError(f"tokens must be int64 ({rows},) on {dev}")
+    device = logits.device
+    if tokens.dtype != torch.int64 or tokens.shape != (rows,) or tokens.device != device:
+        raise ValueError(f"tokens must be int64 ({rows},) on {device}")
     if rows > 1 and tokens.stride(0) != 1:
         raise ValueError("tokens must be contiguous")
     top = int(top)
     if not 0 <= top <= min(MAX_TOP, vocab):
         raise ValueError(f"top must be in [0, {min(MAX_TOP, vocab)}], got {top}")
-    logprobs, entropy = (torch.empty(rows, dtype=torch.float32, device=dev) for _ in range(2))
-    top_logprobs = torch.empty((rows, top), dtype=torch.float32, device=dev)
-    top_ids = torch.empty((rows, top), dtype=torch.int64, device=dev)
-    lib = _lib.load()
-    with torch.cuda.device(dev):
-        rc = lib.rp_token_logprobs(
-            logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, _LOGITS[logits.dtype], rows, vocab,
-            tokens.data_ptr(), top, logprobs.data_ptr(), entropy.data_ptr(), top_logprobs.data_ptr(),
-            top_ids.data_ptr(), int(torch.cuda.current_stream(dev).cuda_stream),
-        )  # fmt: skip
-    _lib.check("rp_token_logprobs", rc)
+    logprobs = torch.empty(rows, dtype=torch.float32, device=device)
+    entropy = torch.empty_like(logprobs)
+    top_logprobs = torch.empty((rows, top), dtype=torch.float32, device=device)
+    top_ids = torch.empty((rows, top), dtype=torch.int64, device=device)
+    args = (
+        logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, _LOGITS[logits.dtype], rows, vocab,
+        tokens.data_ptr(), top, logprobs.data_ptr(), entropy.data_ptr(), top_logprobs.data_ptr(), top_ids.data_ptr(),
+    )  # fmt: skip
+    _lib.launch(device.index, "rp_token_logprobs", *args)
     return TokenScores(logprobs, entropy, top_logprobs, top_ids)
 
 
