@@ -15,8 +15,10 @@
 // its product with x - ref in fp32; the maximum is not needed exactly.
 // Alternatives cost the pass nothing but a running maximum: each thread leaves
 // the maxima of its segments (32 to a few hundred values) in shared memory.
-// Afterwards the k-th largest of 128 group maxima is a lower bound of the k-th
-// largest value, and the few segments that reach it are read again (from L2).
+// Afterwards the k-th largest of 32 to 128 group maxima is a lower bound of the
+// k-th largest value, and the few segments that reach it are read again (from
+// L2).  A thread brings its own vectors in through a ring of its own (16-byte
+// cp.async, two batches ahead), which needs no barrier and no registers.
 // Few rows are split over a cluster of CTAs, joined through distributed shared
 // memory: one launch, no workspace.
 #include <cooperative_groups.h>
@@ -34,12 +36,14 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kT = 256;              // threads of a CTA
-constexpr int kU = 4;                // 16-byte vectors a thread has in flight
-constexpr int kGroups = 128;         // groups whose maxima bound the k-th value
+constexpr int kT = 128;              // threads of a CTA
+constexpr int kU = 4;                // 16-byte vectors of a thread's batch
+constexpr int kStages = 3;           // batches of a thread in shared memory
+constexpr int kRing = kStages * kU * kT * 16;  // bytes: 24 KB, six CTAs an SM
 constexpr int kSegments = 16;        // segments of a thread, at most
-constexpr int kCandidates = 2048;    // values kept for the selection
+constexpr int kCandidates = 2048;    // values kept for the selection (in the ring's place)
 constexpr int kMaxCluster = 8;
+static_assert(kCandidates * 8 + kSegments * kT * 2 <= kRing && kMaxTop <= kT, "");
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kHeadroom = 6.9f;    // the reference may lie 2^10 below a value
@@ -101,6 +105,26 @@ struct Type {
   }
 };
 
+// A vector with elements missing, -inf there: elements e0, e0 + 1, ... of a row
+// of V.  (Not inlined: the pass has it four times, for two vectors a row.)
+template <int DT>
+__device__ __noinline__ uint4 edge_vector(const char* row, int e0, int V) {
+  using E = Type<DT>;
+  uint32_t w[4] = {E::kNegInf, E::kNegInf, E::kNegInf, E::kNegInf};
+#pragma unroll
+  for (int i = 0; i < E::kVec; ++i) {
+    const int e = e0 + i;
+    if (e < 0 || e >= V) continue;
+    if constexpr (DT == 2) {
+      w[i] = __ldg(reinterpret_cast<const uint32_t*>(row) + e);
+    } else {
+      const uint32_t u = __ldg(reinterpret_cast<const uint16_t*>(row) + e);
+      w[i / 2] = i % 2 ? (w[i / 2] & 0xffffu) | (u << 16) : (w[i / 2] & 0xffff0000u) | u;
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // Sums over a set of values relative to ref: l = sum e^(x - ref), s = sum
 // e^(x - ref) log2(e) (x - ref).
 struct Sums {
@@ -127,9 +151,11 @@ __device__ __forceinline__ Sums joined(Sums a, Sums b) {
 struct Shared {
   Sums warp_sums[kT / 32];
   Sums sums;                        // of this CTA
-  uint32_t groups[kGroups];         // keys of the group maxima
+  uint4 groups[kT / 4];             // keys of the groups' maxima
   uint64_t best[kMaxTop];           // this CTA's alternatives
   uint64_t merged[kMaxCluster * kMaxTop];
+  int votes[kT / 32];
+  int hits;
   int count, picked;
   uint32_t bound;
 };
@@ -138,7 +164,7 @@ struct Shared {
 // may be reordered.  All threads of the CTA.
 __device__ void select_top(uint64_t* keys, int n, int k, uint64_t* out, Shared& sh) {
   __syncthreads();
-  if (n > kT) {
+  if (n > 4 * kT) {
     // the k-th largest, bit by bit, and what lies at or above it to the front
     uint64_t thr = 0;
     for (int bit = 63; bit >= 0; --bit) {
@@ -163,9 +189,10 @@ __device__ void select_top(uint64_t* keys, int n, int k, uint64_t* out, Shared& 
     n = k;
     __syncthreads();
   }
-  if (threadIdx.x < n) {
-    const uint64_t key = keys[threadIdx.x];
+  for (int j = threadIdx.x; j < n; j += kT) {
+    const uint64_t key = keys[j];
     int rank = 0;
+#pragma unroll 8
     for (int i = 0; i < n; ++i) rank += keys[i] > key;
     if (rank < k) out[rank] = key;
   }
@@ -174,13 +201,15 @@ __device__ void select_top(uint64_t* keys, int n, int k, uint64_t* out, Shared& 
 
 // One row per cluster; the CTAs of a cluster take equal parts of it.
 template <int DT>
-__global__ void __launch_bounds__(kT, 4) score_kernel(const ScoreArgs a, int per_segment) {
+__global__ void __launch_bounds__(kT, 6) score_kernel(const ScoreArgs a, int per_segment) {
   using E = Type<DT>;
   constexpr int kVec = E::kVec;
-  extern __shared__ uint64_t dynamic[];  // with alternatives: candidates, then segment maxima
+  // the ring, whose place the candidates take later; with alternatives, segment maxima
+  extern __shared__ __align__(16) uint8_t dynamic[];
   __shared__ Shared sh;
-  uint64_t* cand = dynamic;
-  float* segs = reinterpret_cast<float*>(dynamic + kCandidates);
+  uint64_t* cand = reinterpret_cast<uint64_t*>(dynamic);
+  uint16_t* hit_list = reinterpret_cast<uint16_t*>(cand + kCandidates);  // segments that reach the bound
+  float* segs = reinterpret_cast<float*>(dynamic + kRing);
   const cg::cluster_group cluster = cg::this_cluster();
   const int parts = static_cast<int>(cluster.num_blocks()), part = static_cast<int>(cluster.block_rank());
   const int r = blockIdx.x / parts, t = threadIdx.x, warp = t >> 5, lane = t & 31;
@@ -195,24 +224,18 @@ __global__ void __launch_bounds__(kT, 4) score_kernel(const ScoreArgs a, int per
   const int v0 = static_cast<int>(static_cast<int64_t>(vectors) * part / parts);
   const int v1 = static_cast<int>(static_cast<int64_t>(vectors) * (part + 1) / parts);
   const int inner0 = shift ? 1 : 0, inner1 = (V + shift) / kVec;  // whole vectors
-  const auto edge = [&](int v) {  // a vector with elements missing: -inf there
-    uint32_t w[4] = {E::kNegInf, E::kNegInf, E::kNegInf, E::kNegInf};
+  uint4* ring = reinterpret_cast<uint4*>(dynamic) + t;  // (stage, vector) at ring[(stage * kU + u) * kT]
+  const auto fill = [&](int stage, int v) {  // the batch that starts with vector v
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      const int e = v * kVec - shift + i;
-      if (e < 0 || e >= V) continue;
-      if constexpr (DT == 2) {
-        w[i] = __ldg(reinterpret_cast<const uint32_t*>(row) + e);
-      } else {
-        const uint32_t u = __ldg(reinterpret_cast<const uint16_t*>(row) + e);
-        w[i / 2] = i % 2 ? (w[i / 2] & 0xffffu) | (u << 16) : (w[i / 2] & 0xffff0000u) | u;
-      }
+    for (int u = 0; u < kU && v < v1; ++u) {
+      uint4* dst = ring + (stage * kU + u) * kT;
+      const int w = v + u * kT;
+      if (w >= inner0 && w < min(inner1, v1))
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(base + w) : "memory");
+      else
+        *dst = w < v1 ? edge_vector<DT>(row, w * kVec - shift, V) : make_uint4(E::kNegInf, E::kNegInf, E::kNegInf, E::kNegInf);
     }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-  };
-  const auto load = [&](int v) {
-    if (v >= inner0 && v < inner1) return __ldcs(base + v);
-    return edge(v);
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
 
   // ---- the pass
@@ -220,11 +243,16 @@ __global__ void __launch_bounds__(kT, 4) score_kernel(const ScoreArgs a, int per
   float seg = -INFINITY, best = -INFINITY;
   int in_seg = 0, n_seg = 0;
   uint64_t l2 = 0, s2 = 0;
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) fill(i, v0 + t + i * kU * kT);
+  int stage = 0;
   for (int v = v0 + t; v < v1; v += kU * kT) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
     uint4 x[kU];
 #pragma unroll
-    for (int u = 0; u < kU; ++u)
-      x[u] = v + u * kT < v1 ? load(v + u * kT) : make_uint4(E::kNegInf, E::kNegInf, E::kNegInf, E::kNegInf);
+    for (int u = 0; u < kU; ++u) x[u] = ring[(stage * kU + u) * kT];
+    fill(stage == 0 ? kStages - 1 : stage - 1, v + (kStages - 1) * kU * kT);
+    stage = stage == kStages - 1 ? 0 : stage + 1;
     uint32_t m = x[0].x;
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
@@ -296,39 +324,51 @@ __global__ void __launch_bounds__(kT, 4) score_kernel(const ScoreArgs a, int per
       segs[n_seg++ * kT + t] = seg;
       best = max_nan(best, seg);
     }
+    // the k-th largest of the maxima of 2 k or more groups of lanes (32, 64 or 128 groups)
+    const int lanes = k <= 16 ? kT / 32 : k <= 32 ? kT / 64 : 1;  // of a group
     float g = best;
-#pragma unroll
-    for (int s = 1; s < kT / kGroups; s *= 2) g = max_nan(g, __shfl_xor_sync(0xffffffffu, g, s));
-    if (t % (kT / kGroups) == 0) sh.groups[t / (kT / kGroups)] = value_key(g);
+    for (int s = 1; s < lanes; s *= 2) g = max_nan(g, __shfl_xor_sync(0xffffffffu, g, s));
+    const uint32_t group_key = value_key(g);
+    if (t % lanes == 0) reinterpret_cast<uint32_t*>(sh.groups)[t / lanes] = group_key;
     if (t == 0) {
       sh.count = 0;
+      sh.hits = 0;
       sh.bound = 0;
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");  // the ring's place is free
     __syncthreads();
-    if (t < kGroups) {
-      const uint32_t key = sh.groups[t];
+    if (t < kT / lanes) {
+      const uint32_t key = reinterpret_cast<const uint32_t*>(sh.groups)[t];
       int above = 0;
-      for (int i = 0; i < kGroups; ++i) above += sh.groups[i] > key || (sh.groups[i] == key && i < t);
+#pragma unroll 4
+      for (int i = 0; i < kT / lanes / 4; ++i) {
+        const uint4 o = sh.groups[i];
+        above += (o.x > key || (o.x == key && 4 * i < t)) + (o.y > key || (o.y == key && 4 * i + 1 < t)) +
+                 (o.z > key || (o.z == key && 4 * i + 2 < t)) + (o.w > key || (o.w == key && 4 * i + 3 < t));
+      }
       if (above == k - 1) sh.bound = key;
     }
     __syncthreads();
-    // candidates: every value at or above the bound; `strict`: above it
+    // candidates: every value at or above the bound; `strict`: above it.  The
+    // segments that reach it are listed first; then a warp reads one at a time.
     const auto collect = [&](uint32_t bound, bool strict) {
       for (int i = 0; i < n_seg; ++i) {
         const uint32_t sk = value_key(segs[i * kT + t]);
-        if (strict ? sk <= bound : sk < bound) continue;
-        for (int j = 0; j < per_segment * kU; ++j) {
-          const int v = v0 + t + (i * per_segment * kU + j) * kT;
-          if (v >= v1) break;
-          for (int c = 0; c < kVec; ++c) {
-            const int e = v * kVec - shift + c;
-            if (e < 0 || e >= V) continue;
-            const float x = E::at(row, e);
-            const uint32_t key = value_key(x);
-            if (strict ? key <= bound : key < bound) continue;
-            const int at = atomicAdd(&sh.count, 1);
-            if (at < kCandidates) cand[at] = rank_key(x, e);
-          }
+        if (strict ? sk > bound : sk >= bound) hit_list[atomicAdd(&sh.hits, 1)] = static_cast<uint16_t>(i * kT + t);
+      }
+      __syncthreads();
+      const int hits = sh.hits, each = per_segment * kU * kVec;
+      for (int i = warp; i < hits; i += kT / 32) {
+        const int hit = hit_list[i], first = v0 + hit % kT + hit / kT * per_segment * kU * kT;
+#pragma unroll 1
+        for (int j = lane; j < each; j += 32) {
+          const int v = first + j / kVec * kT, e = v * kVec - shift + j % kVec;
+          if (v >= v1 || e < 0 || e >= V) continue;
+          const float y = E::at(row, e);
+          const uint32_t key = value_key(y);
+          if (strict ? key <= bound : key < bound) continue;
+          const int at = atomicAdd(&sh.count, 1);
+          if (at < kCandidates) cand[at] = rank_key(y, e);
         }
       }
       __syncthreads();
@@ -340,7 +380,7 @@ __global__ void __launch_bounds__(kT, 4) score_kernel(const ScoreArgs a, int per
     // Too many: the values above the bound alone.  Are these too many as well,
     // the k-th largest of those at hand is a higher bound.
     while (n > kCandidates) {
-      if (t == 0) sh.count = 0;
+      if (t == 0) sh.count = sh.hits = 0;
       __syncthreads();
       collect(bound, true);
       n = sh.count;
@@ -348,7 +388,7 @@ __global__ void __launch_bounds__(kT, 4) score_kernel(const ScoreArgs a, int per
       if (n > kCandidates) {
         select_top(cand, kCandidates, k, sh.best, sh);
         bound = static_cast<uint32_t>(sh.best[k - 1] >> 32);
-        if (t == 0) sh.count = 0;
+        if (t == 0) sh.count = sh.hits = 0;
         __syncthreads();
         collect(bound, false);
         n = sh.count;
@@ -360,12 +400,12 @@ __global__ void __launch_bounds__(kT, 4) score_kernel(const ScoreArgs a, int per
         for (int e = e0; e < e1 && need > 0; e += kT) {
           const bool tie = e + t < e1 && value_key(E::at(row, e + t)) == bound;
           const uint32_t votes = __ballot_sync(0xffffffffu, tie);
-          if (lane == 0) sh.groups[warp] = __popc(votes);
+          if (lane == 0) sh.votes[warp] = __popc(votes);
           __syncthreads();
           int before = __popc(votes & ((1u << lane) - 1)), all = 0;
           for (int w = 0; w < kT / 32; ++w) {
-            if (w < warp) before += sh.groups[w];
-            all += sh.groups[w];
+            if (w < warp) before += sh.votes[w];
+            all += sh.votes[w];
           }
           if (tie && before < need) cand[n + before] = rank_key(key_value(bound), e + t);
           n += min(all, need);
@@ -385,7 +425,6 @@ __global__ void __launch_bounds__(kT, 4) score_kernel(const ScoreArgs a, int per
   }
 
   // ---- the parts joined by the cluster's first CTA
-  uint64_t* best_keys = sh.best;
   if (parts > 1) {
     cluster.sync();
     if (part == 0 && top > 0) {
@@ -397,8 +436,7 @@ __global__ void __launch_bounds__(kT, 4) score_kernel(const ScoreArgs a, int per
         n += m;
       }
       __syncthreads();
-      select_top(sh.merged, n, top, cand, sh);
-      best_keys = cand;
+      select_top(sh.merged, n, top, sh.best, sh);
     }
   } else {
     __syncthreads();
@@ -421,7 +459,7 @@ __global__ void __launch_bounds__(kT, 4) score_kernel(const ScoreArgs a, int per
       a.entropy[r] = nothing ? 0.f : logl - kLn2 * (all.s / all.l);
     }
     for (int i = t; i < top; i += kT) {
-      const uint64_t key = best_keys[i];
+      const uint64_t key = sh.best[i];
       a.top_ids[static_cast<int64_t>(r) * top + i] = 0xffffffffu - static_cast<uint32_t>(key);
       a.top_logprobs[static_cast<int64_t>(r) * top + i] =
           nothing ? -INFINITY : (key_value(static_cast<uint32_t>(key >> 32)) - ref) - logl;
@@ -432,17 +470,18 @@ __global__ void __launch_bounds__(kT, 4) score_kernel(const ScoreArgs a, int per
 
 template <int DT>
 cudaError_t launch(const ScoreArgs& a, cudaStream_t st) {
-  // CTAs of a row: enough for four CTAs an SM, with at least 1024 vectors each.
+  // CTAs of a row: while the GPU holds all of them at once (six an SM) and each has two vectors a
+  // thread.
   constexpr int kVec = Type<DT>::kVec;
   const int64_t vectors = static_cast<int64_t>(a.vocab) / kVec + 2;
   int parts = 1;
-  while (parts < kMaxCluster && static_cast<int64_t>(a.rows) * parts * 2 <= 148 * 4 &&
-         vectors / (parts * 2) >= kT)
+  while (parts < kMaxCluster && static_cast<int64_t>(a.rows) * parts * 2 <= 148 * 6 &&
+         vectors / (parts * 2) >= 2 * kT)
     parts *= 2;
   const int64_t batches = (vectors / parts + 1 + kU * kT - 1) / (kU * kT);  // of a thread
   const int per_segment = static_cast<int>((batches + kSegments - 1) / kSegments);
   const int64_t segments = (batches + per_segment - 1) / per_segment;
-  const size_t smem = a.top > 0 ? kCandidates * 8 + static_cast<size_t>(segments) * kT * 4 : 0;
+  const size_t smem = kRing + (a.top > 0 ? static_cast<size_t>(segments) * kT * 4 : 0);
   if (static_cast<int64_t>(a.rows) * parts > 0x7FFFFFFF) return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(a.rows) * parts);

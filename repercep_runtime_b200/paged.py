@@ -274,7 +274,7 @@ def decode(
     ws = torch.empty(need, dtype=torch.uint8, device=device)
     _lib.launch(
         device.index, "rp_paged_decode", byref(cache._struct()), q.data_ptr(), _I64x2(q0, q1), _HALF[dtype], B, Hq,
-        page_table.data_ptr(), row, pages, lengths.data_ptr(), 0.0 if scale is None else scale,
+        page_table.data_ptr(), row, pages, lengths.data_ptr(), 0.0 if scale is None else float(scale),
         out.data_ptr(), _I64x2(o0, o1), None if lse is None else lse.data_ptr(), w, w_strides, w_cols,
         ws.data_ptr(), need,
     )  # fmt: skip
