@@ -200,19 +200,19 @@ __device__ __forceinline__ float key_weight(uint32_t k) {
 // count and place what is kept in order, so ties at the threshold go to the
 // lowest positions.  Reads each weight from HBM once; bound by the latency of
 // its few dependent passes, which the split over a cluster shortens.
-constexpr int kSelThreads = 512;
+constexpr int kSelThreads = 256;
 constexpr int kSelWarps = kSelThreads / 32;
+static_assert(kSelThreads >= 256, "a thread for every sum of 8 bins");
 constexpr int kSelBatch = 8;  // keys of a thread in flight
 constexpr int kBins = 2048;
 constexpr int kCoarse = kBins / 8;
-constexpr int kSelCluster = 8;         // CTAs of a row, at most
-constexpr int kSliceAim = 8192;        // positions of a CTA that a larger cluster is not taken for
+constexpr int kSelCluster = 16;        // CTAs of a row, at most (8 where a GPU cannot hold 16)
+constexpr int kSliceAim = 4096;        // positions of a CTA that a larger cluster is not taken for
 constexpr int kSliceHeld = 44 * 1024;  // positions of a CTA held in shared memory, at most
 
 struct SelectShared {
   int4 hist[3][kBins / 4];
   int4 coarse[3][kCoarse / 4];
-  int4 all[kSelCluster][kCoarse / 4];
   int above[kSelWarps], ties[kSelWarps];  // of each warp's run
   int part_above, part_ties;              // of this CTA's slice
   int scan[kSelWarps];
@@ -229,6 +229,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
   const int parts = static_cast<int>(cluster.num_blocks()), part = static_cast<int>(cluster.block_rank());
   const int h = blockIdx.x / parts, b = blockIdx.y, H = a.kv.heads;
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  launch_next();
   const int n = table_length(a.t, a.kv.page_size, b, a.status);
   const int keep = min(n, a.budget);
   const float* w = a.weights.w + b * a.weights.s_seq + h * a.weights.s_head;
@@ -299,15 +300,12 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
     }
     if (parts > 1) cluster.sync();
     else __syncthreads();
-    if (t < parts * (kCoarse / 4)) {
-      const int q = t / (kCoarse / 4), quad = t % (kCoarse / 4);
-      sh.all[q][quad] = cluster.map_shared_rank(&sh, q)->coarse[pass][quad];
-    }
-    __syncthreads();
     // a sum of 8 bins a thread, from the top: the one in which the running count reaches `left`
     int c = 0, before = 0;
     if (t < kCoarse) {
-      for (int i = 0; i < parts; ++i) c += reinterpret_cast<const int*>(sh.all[i])[kCoarse - 1 - t];
+#pragma unroll
+      for (int q = 0; q < kSelCluster; ++q)
+        if (q < parts) c += reinterpret_cast<const int*>(cluster.map_shared_rank(&sh, q)->coarse[pass])[kCoarse - 1 - t];
       before = c;
 #pragma unroll
       for (int s = 1; s < 32; s *= 2) {
@@ -327,14 +325,15 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
       }
     }
     __syncthreads();
-    // its bins, by one warp: lane i sums bin 7 - i % 8 over two of the CTAs
+    // its bins, by one warp: lane i sums bin 7 - i % 8 over every fourth CTA
     if (warp == 0) {
       const int group = sh.digit, rest = sh.left, bin = group * 8 + 7 - (lane & 7);
-      int n0 = 0, n1 = 0;
-      const int q0 = lane >> 3, q1 = q0 + 4;
-      if (q0 < parts) n0 = reinterpret_cast<const int*>(cluster.map_shared_rank(&sh, q0)->hist[pass])[bin];
-      if (q1 < parts) n1 = reinterpret_cast<const int*>(cluster.map_shared_rank(&sh, q1)->hist[pass])[bin];
-      int m = n0 + n1;
+      int m = 0;
+#pragma unroll
+      for (int i = 0; i < kSelCluster / 4; ++i) {
+        const int q = (lane >> 3) + 4 * i;
+        if (q < parts) m += reinterpret_cast<const int*>(cluster.map_shared_rank(&sh, q)->hist[pass])[bin];
+      }
       m += __shfl_xor_sync(0xffffffffu, m, 8);
       m += __shfl_xor_sync(0xffffffffu, m, 16);
       int run = m;
@@ -440,6 +439,7 @@ __global__ void __launch_bounds__(kMoveWarps * 32) evict_move_kernel(const Evict
   const int j0 = (blockIdx.x * kMoveWarps + (threadIdx.x >> 5)) * kMoveRows, h = blockIdx.y, b = blockIdx.z;
   const int H = a.kv.heads;
   const int j = j0 + lane;
+  wait_previous();
   const int p = lane < kMoveRows && j < a.budget ? a.kept[(static_cast<int64_t>(b) * H + h) * a.budget + j] : -1;
   int64_t from = -1, to = -1;
   if (p >= 0) {
@@ -479,6 +479,28 @@ __global__ void __launch_bounds__(kMoveWarps * 32) evict_move_kernel(const Evict
     }
 }
 
+// Clusters of 16 CTAs are allowed if the device can hold one of them.
+template <typename F>
+cudaError_t select_clusters(F* kernel, size_t smem, int* most) {
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(kSelCluster);
+  cfg.blockDim = dim3(kSelThreads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = kSelCluster;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int clusters = 0;
+  e = cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg);
+  if (e != cudaSuccess) return e;
+  *most = clusters > 0 ? kSelCluster : kSelCluster / 2;
+  return cudaSuccess;
+}
+
 }  // namespace
 
 cudaError_t launch_paged_append(const AppendArgs& a, cudaStream_t st) {
@@ -492,23 +514,28 @@ cudaError_t launch_paged_append(const AppendArgs& a, cudaStream_t st) {
 }
 
 cudaError_t launch_paged_evict(const EvictArgs& a, cudaStream_t st) {
+  static std::atomic<int> most_parts[kMaxDevices];  // CTAs of a cluster, once this device is set up
+  const int dev = current_device();
+  int most = most_parts[dev].load(std::memory_order_relaxed);
+  if (most == 0) {
+    cudaError_t e = cudaFuncSetAttribute(evict_select_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         kSliceHeld * 4);
+    if (e == cudaSuccess) e = select_clusters(evict_select_kernel<true>, kSliceHeld * 4, &most);
+    int other = 0;
+    if (e == cudaSuccess) e = select_clusters(evict_select_kernel<false>, 0, &other);
+    if (e != cudaSuccess) return e;
+    if (other < most) most = other;
+    most_parts[dev].store(most, std::memory_order_relaxed);
+  }
   const int64_t cap = static_cast<int64_t>(a.t.pages) * a.kv.page_size;
   int parts = 1;
-  // a larger cluster while the slices are long and the GPU holds all CTAs at once
-  while (parts < kSelCluster && cap > static_cast<int64_t>(parts) * kSliceAim &&
-         static_cast<int64_t>(a.kv.heads) * a.t.B * parts * 2 <= 148 * 4)
+  // a larger cluster while the slices are long and the GPU holds all CTAs at once (five an SM)
+  while (parts < most && cap > static_cast<int64_t>(parts) * kSliceAim &&
+         static_cast<int64_t>(a.kv.heads) * a.t.B * parts * 2 <= 148 * 5)
     parts *= 2;
   const int64_t per = (cap + parts - 1) / parts;
   const bool held = per <= kSliceHeld;
   if (static_cast<int64_t>(a.kv.heads) * parts > 0x7FFFFFFF) return cudaErrorInvalidValue;
-  static std::atomic<bool> ready[kMaxDevices];
-  const int dev = current_device();
-  if (!ready[dev].load(std::memory_order_relaxed)) {
-    const cudaError_t e = cudaFuncSetAttribute(evict_select_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               kSliceHeld * 4);
-    if (e != cudaSuccess) return e;
-    ready[dev].store(true, std::memory_order_relaxed);
-  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(a.kv.heads * parts, a.t.B);
   cfg.blockDim = dim3(kSelThreads);
@@ -526,14 +553,13 @@ cudaError_t launch_paged_evict(const EvictArgs& a, cudaStream_t st) {
   constexpr int kRows = kMoveRows * kMoveWarps;
   const dim3 grid((a.budget + kRows - 1) / kRows, a.kv.heads, a.t.B);
   switch (a.kv.D * (a.kv.dtype == kKvE4m3 ? 1 : 2)) {
-    case 32: evict_move_kernel<32><<<grid, kMoveWarps * 32, 0, st>>>(a); break;
-    case 64: evict_move_kernel<64><<<grid, kMoveWarps * 32, 0, st>>>(a); break;
-    case 128: evict_move_kernel<128><<<grid, kMoveWarps * 32, 0, st>>>(a); break;
-    case 256: evict_move_kernel<256><<<grid, kMoveWarps * 32, 0, st>>>(a); break;
-    case 512: evict_move_kernel<512><<<grid, kMoveWarps * 32, 0, st>>>(a); break;
+    case 32: return launch_after(evict_move_kernel<32>, grid, kMoveWarps * 32, 0, st, a);
+    case 64: return launch_after(evict_move_kernel<64>, grid, kMoveWarps * 32, 0, st, a);
+    case 128: return launch_after(evict_move_kernel<128>, grid, kMoveWarps * 32, 0, st, a);
+    case 256: return launch_after(evict_move_kernel<256>, grid, kMoveWarps * 32, 0, st, a);
+    case 512: return launch_after(evict_move_kernel<512>, grid, kMoveWarps * 32, 0, st, a);
     default: return cudaErrorInvalidValue;
   }
-  return cudaGetLastError();
 }
 
 }  // namespace rp

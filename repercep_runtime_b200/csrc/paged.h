@@ -136,6 +136,28 @@ inline int current_device() {
 }
 
 #ifdef __CUDACC__
+// Programmatic launches: what follows may be launched; what came before is
+// complete and its memory visible.
+__device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// A launch that may begin while the launch before it ends (its kernel waits
+// for that one's end itself).
+template <typename F, typename A>
+cudaError_t launch_after(F* kernel, dim3 grid, int threads, size_t smem, cudaStream_t st, const A& arg) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, arg);
+}
+
 // Length of sequence b, held to what its page table can address.
 __device__ __forceinline__ int table_length(const PagedTable& t, int page_size, int b, int* status) {
   const int n = t.lengths[b];

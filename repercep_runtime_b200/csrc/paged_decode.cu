@@ -169,11 +169,6 @@ __device__ __forceinline__ uint16_t round16(float x, bool f16) {
 }
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
 
-// Programmatic launches: what follows may be launched; what came before is
-// complete and its memory visible.
-__device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 // A place in the line of tiles: sequence, item of the sequence (KV head and
 // column group), tile of the item.
 struct Place {
@@ -847,22 +842,6 @@ __global__ void __launch_bounds__(256) decode_weights_kernel(const Params p) {
         if (j + i < n) dst[j + i] = old[i] + w[i];
     }
   }
-}
-
-// A launch that may begin while the launch before it ends (it waits for it).
-template <typename F, typename A>
-cudaError_t launch_after(F* kernel, dim3 grid, int threads, size_t smem, cudaStream_t st, const A& arg) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, arg);
 }
 
 int sm_count(int dev) {
