@@ -529,9 +529,9 @@ cudaError_t launch_paged_evict(const EvictArgs& a, cudaStream_t st) {
   }
   const int64_t cap = static_cast<int64_t>(a.t.pages) * a.kv.page_size;
   int parts = 1;
-  // a larger cluster while the slices are long and the GPU holds all CTAs at once (five an SM)
+  // a larger cluster while the slices are long and the GPU holds all CTAs at once (three an SM)
   while (parts < most && cap > static_cast<int64_t>(parts) * kSliceAim &&
-         static_cast<int64_t>(a.kv.heads) * a.t.B * parts * 2 <= 148 * 5)
+         static_cast<int64_t>(a.kv.heads) * a.t.B * parts * 2 <= 148 * 3)
     parts *= 2;
   const int64_t per = (cap + parts - 1) / parts;
   const bool held = per <= kSliceHeld;

@@ -99,8 +99,16 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool read) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(read ? 16 : 0)
+// Cached rows leave L2 first: they are read once, while the scores and weights
+// that a later launch reads stay.
+__device__ __forceinline__ uint64_t evict_first() {
+  uint64_t policy;
+  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+  return policy;
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool read, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src),
+               "r"(read ? 16 : 0), "l"(policy)
                : "memory");
 }
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool read) {
@@ -281,6 +289,7 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
 
   // ---- loads: lane's key of the warp's slice, its page id one step ahead
   const int my_key = lane % C::kKeys, my_col = lane % C::kChunks;
+  const uint64_t policy = evict_first();
   const uint8_t* k_col = kv.k + my_col * 16;
   const uint8_t* v_col = kv.v + my_col * 16;
   int page = 0;
@@ -330,8 +339,8 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
           constexpr int kRsh = C::kRow >= 128 ? 0 : C::kRow == 64 ? 1 : 2;
           constexpr int kMask = C::kChunks >= 8 ? 7 : C::kChunks - 1;
           const uint32_t dst = base + r * C::kRow + ((my_col ^ ((r >> kRsh) & kMask)) << 4);
-          cp_async16(dst, k_col + o, read);
-          cp_async16(dst + C::kRowsBytes, v_col + o, read);
+          cp_async16(dst, k_col + o, read, policy);
+          cp_async16(dst + C::kRowsBytes, v_col + o, read, policy);
         }
       }
       --to_load;
