@@ -479,3 +479,50 @@ def fp8_attention_bshd_op(
 @fp8_attention_bshd_op.register_fake
 def _fp8_attention_bshd_fake(q, k, v, causal=False, scale=0.0, scale_mode=0, p_mode=0):  # type: ignore[no-untyped-def]
     return torch.empty_like(q)
+
+
+@torch.library.custom_op("repercep_b200::paged_decode", mutates_args=())
+def paged_decode_op(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    page_table: torch.Tensor,
+    lengths: torch.Tensor,
+    k_scales: torch.Tensor | None = None,
+    v_scales: torch.Tensor | None = None,
+    layout: str = "bhsd",
+    scale: float = 0.0,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """``torch.ops.repercep_b200.paged_decode`` — attention of one new token per
+    sequence over a page pool (``paged.PagedKV``'s tensors); out and lse."""
+    from . import paged
+
+    cache = paged.PagedKV(k, v, k_scales, v_scales, layout)
+    return paged.decode(q, cache, page_table, lengths, scale=scale if scale > 0 else None, return_lse=True)
+
+
+@paged_decode_op.register_fake
+def _paged_decode_fake(q, k, v, page_table, lengths, k_scales=None, v_scales=None, layout="bhsd", scale=0.0):  # type: ignore[no-untyped-def]
+    return q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32)
+
+
+@torch.library.custom_op("repercep_b200::token_logprobs", mutates_args=())
+def token_logprobs_op(
+    logits: torch.Tensor, tokens: torch.Tensor, top: int = 0
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``torch.ops.repercep_b200.token_logprobs`` — log probabilities of the
+    tokens, entropies, top log probabilities and their ids."""
+    from . import scoring
+
+    return tuple(scoring.token_logprobs(logits, tokens, top=top))
+
+
+@token_logprobs_op.register_fake
+def _token_logprobs_fake(logits, tokens, top=0):  # type: ignore[no-untyped-def]
+    rows = logits.shape[0]
+    return (
+        logits.new_empty(rows, dtype=torch.float32),
+        logits.new_empty(rows, dtype=torch.float32),
+        logits.new_empty((rows, top), dtype=torch.float32),
+        logits.new_empty((rows, top), dtype=torch.int64),
+    )

@@ -444,3 +444,57 @@ def test_refusals():
     assert paged.evict(cache, empty, none, torch.zeros((0, 2, 48), device="cuda"), empty, budget=4, recent=1).kept.shape == (0, 2, 4)
     flat = torch.zeros((2, 0), dtype=torch.int32, device="cuda")
     assert bool((paged.decode(q, cache, flat, torch.zeros_like(n)) == 0).all())
+
+
+# --------------------------------------------------------------- other ways
+def test_op_custom_op_and_graph_capture_agree():
+    from repercep_runtime_b200 import ops, paged, scoring  # noqa: F401
+    from repercep_runtime_b200.attention import PagedDecode
+
+    cache, table, n, _, _ = filled([300, 7, 0, 65], 2, 16, 128, "e4m3", seed=61)
+    q = rows((4, 8, 128), torch.bfloat16, 62)
+    op = PagedDecode()
+    assert op.available and op.supports(8, 2, 128) and not op.supports(8, 3, 128) and not op.supports(8, 2, 96)
+    out, lse = op(q, cache, table, n, return_lse=True)
+    got = torch.ops.repercep_b200.paged_decode(q, cache.k, cache.v, table, n, cache.k_scales, cache.v_scales)
+    assert torch.equal(got[0], out) and torch.equal(got[1], lse)
+
+    # append, decode with weights, evict and scores captured in one graph and replayed on new inputs
+    weights = torch.zeros((4, 2, table.shape[1] * 16), device="cuda")
+    wide, _ = make_table([301, 8, 1, 66], 16, table.shape[1] + 1, seed=61)
+    pages = int(wide[wide < 1000].max()) + 1
+    cut, extra = make_table([40, 8, 1, 40], 16, 3, first=pages)
+    pool = make_cache(pages + extra, 2, 16, 128, "e4m3")
+    lengths = torch.zeros(4, dtype=torch.int32, device="cuda")
+    k, v = rows((372, 2, 128), torch.bfloat16, 63), rows((372, 2, 128), torch.bfloat16, 64)
+    starts = torch.tensor([0, 300, 307, 307, 372], dtype=torch.int32, device="cuda")
+    lengths = paged.append(pool, k, v, wide, lengths, starts=starts)
+    weights = torch.zeros((4, 2, wide.shape[1] * 16), device="cuda")
+    logits, tokens = rows((4, 5000), torch.bfloat16, 65), torch.tensor([1, 2, 3, 4999], device="cuda")
+    new = rows((4, 2, 128), torch.bfloat16, 66)
+
+    def step():
+        after = paged.append(pool, new, new, wide, lengths, weights=weights)
+        out, lse = paged.decode(q, pool, wide, after, weights=weights, return_lse=True)
+        gone = paged.evict(pool, wide, after, weights, cut, budget=40, recent=8)
+        return after, out, lse, *gone, *scoring.token_logprobs(logits, tokens, top=4)
+
+    weights.zero_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    q.copy_(rows((4, 8, 128), torch.bfloat16, 67))
+    new.copy_(rows((4, 2, 128), torch.bfloat16, 68))
+    logits.copy_(rows((4, 5000), torch.bfloat16, 69))
+    weights.zero_()
+    graph.replay()
+    replayed = [t.clone() for t in captured]
+    weights.zero_()
+    for a, b in zip(replayed, step()):
+        assert torch.equal(a, b)
+    check_decode(q, pool, wide, captured[0])
