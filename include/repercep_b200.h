@@ -357,8 +357,9 @@ int rp_paged_decode_workspace_bytes(const rp_paged_kv* kv, int B, int Hq, int ta
  *        execution
  * A sequence of length 0 gives out = 0 and lse = -inf.  sm_scale <= 0 selects
  * 1/sqrt(head_dim).  Scores, sums and accumulators are fp32; softmax weights
- * are rounded to 16 bits for their product with V (fp16 unless the cache is
- * bf16). */
+ * enter their product with V as a 16-bit value and a 16-bit remainder (an e4m3
+ * cache: rounded once, to fp16).  Strides that address more than 2^32 units of
+ * their largest common power of two are refused. */
 int rp_paged_decode(const rp_paged_kv* kv, const void* q, const int64_t* q_strides, int q_dtype,
                     int B, int Hq, const int32_t* page_table, int64_t table_stride,
                     int table_pages, const int32_t* lengths, float sm_scale, void* out,
