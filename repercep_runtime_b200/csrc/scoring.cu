@@ -18,7 +18,9 @@
 // Afterwards the k-th largest of 32 to 128 group maxima is a lower bound of the
 // k-th largest value, and the few segments that reach it are read again (from
 // L2).  A thread brings its own vectors in through a ring of its own (16-byte
-// cp.async, two batches ahead), which needs no barrier and no registers.
+// cp.async, two batches ahead), which needs no barrier and no registers; a CTA
+// that has another row to do starts it there before it selects the last one's
+// alternatives.
 // Few rows are split over a cluster of CTAs, joined through distributed shared
 // memory: one launch, no workspace.
 #include <cooperative_groups.h>
@@ -39,11 +41,16 @@ namespace cg = cooperative_groups;
 constexpr int kT = 128;              // threads of a CTA
 constexpr int kU = 4;                // 16-byte vectors of a thread's batch
 constexpr int kStages = 3;           // batches of a thread in shared memory
-constexpr int kRing = kStages * kU * kT * 16;  // bytes: 24 KB, six CTAs an SM
+constexpr int kRing = kStages * kU * kT * 16;  // bytes: 24 KB, five CTAs an SM
+constexpr int kResident = 5;
+constexpr int kSms = 148;
 constexpr int kSegments = 16;        // segments of a thread, at most
-constexpr int kCandidates = 2048;    // values kept for the selection (in the ring's place)
+constexpr int kCandidates = 512;     // values kept for the selection
+constexpr int kLook = 12;            // values of a thread in flight when segments are read again
+constexpr int kManyHits = 256;       // more segments than this reach a bound only by ties
 constexpr int kMaxCluster = 8;
-static_assert(kCandidates * 8 + kSegments * kT * 2 <= kRing && kMaxTop <= kT, "");
+static_assert(kMaxTop <= kT && kMaxCluster * kMaxTop <= kCandidates, "");
+static_assert(kSegments * kT * 2 <= kMaxCluster * kMaxTop * 8, "the list of segments fits the merged keys");
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kHeadroom = 6.9f;    // the reference may lie 2^10 below a value
@@ -160,35 +167,10 @@ struct Shared {
   uint32_t bound;
 };
 
-// The `k` largest of n different keys, in order, to out[0..k) (n >= k).  keys
-// may be reordered.  All threads of the CTA.
-__device__ void select_top(uint64_t* keys, int n, int k, uint64_t* out, Shared& sh) {
+// The `k` largest of n different keys, in order, to out[0..k) (n >= k), by
+// counting the larger ones of each.  All threads of the CTA.
+__device__ __forceinline__ void select_top(const uint64_t* keys, int n, int k, uint64_t* out) {
   __syncthreads();
-  if (n > 4 * kT) {
-    // the k-th largest, bit by bit, and what lies at or above it to the front
-    uint64_t thr = 0;
-    for (int bit = 63; bit >= 0; --bit) {
-      const uint64_t t = thr | (1ull << bit);
-      int c = 0;
-      for (int i = threadIdx.x; i < n; i += kT) c += keys[i] >= t;
-      c = __reduce_add_sync(0xffffffffu, c);
-      if (threadIdx.x == 0) sh.picked = 0;
-      __syncthreads();
-      if ((threadIdx.x & 31) == 0) atomicAdd(&sh.picked, c);
-      __syncthreads();
-      const bool enough = sh.picked >= k;
-      __syncthreads();
-      if (enough) thr = t;
-    }
-    if (threadIdx.x == 0) sh.picked = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kT)
-      if (keys[i] >= thr) out[atomicAdd(&sh.picked, 1)] = keys[i];
-    __syncthreads();
-    for (int i = threadIdx.x; i < k; i += kT) keys[i] = out[i];
-    n = k;
-    __syncthreads();
-  }
   for (int j = threadIdx.x; j < n; j += kT) {
     const uint64_t key = keys[j];
     int rank = 0;
@@ -199,292 +181,337 @@ __device__ void select_top(uint64_t* keys, int n, int k, uint64_t* out, Shared& 
   __syncthreads();
 }
 
-// One row per cluster; the CTAs of a cluster take equal parts of it.
+// A CTA's part of a row, as vectors that start at 16-byte boundaries: vector v
+// holds elements v * kVec - shift + i, of which the first and last may lack
+// some; [inner0, inner1) are whole, [v0, v1) the part's.
+struct Part {
+  const char* row;
+  const uint4* base;
+  int shift, v0, v1, inner0, inner1;
+};
+
+// One row per cluster at a time; the CTAs of a cluster take equal parts of it.
 template <int DT>
-__global__ void __launch_bounds__(kT, 6) score_kernel(const ScoreArgs a, int per_segment) {
+__global__ void __launch_bounds__(kT, kResident) score_kernel(const ScoreArgs a, int per_segment) {
   using E = Type<DT>;
   constexpr int kVec = E::kVec;
-  // the ring, whose place the candidates take later; with alternatives, segment maxima
-  extern __shared__ __align__(16) uint8_t dynamic[];
+  extern __shared__ __align__(16) uint8_t dynamic[];  // the ring; with alternatives, candidates and segment maxima
   __shared__ Shared sh;
-  uint64_t* cand = reinterpret_cast<uint64_t*>(dynamic);
-  uint16_t* hit_list = reinterpret_cast<uint16_t*>(cand + kCandidates);  // segments that reach the bound
-  float* segs = reinterpret_cast<float*>(dynamic + kRing);
+  uint64_t* cand = reinterpret_cast<uint64_t*>(dynamic + kRing);
+  float* segs = reinterpret_cast<float*>(cand + kCandidates);
+  uint16_t* hit_list = reinterpret_cast<uint16_t*>(sh.merged);  // segments that reach the bound
   const cg::cluster_group cluster = cg::this_cluster();
   const int parts = static_cast<int>(cluster.num_blocks()), part = static_cast<int>(cluster.block_rank());
-  const int r = blockIdx.x / parts, t = threadIdx.x, warp = t >> 5, lane = t & 31;
-  const int V = a.vocab, top = a.top;
-  const char* row = static_cast<const char*>(a.logits) + r * a.stride * E::kSize;
-
-  // The row as vectors that start at 16-byte boundaries: vector v holds
-  // elements v * kVec - shift + i, of which the first and last may lack some.
-  const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15) / E::kSize;
-  const uint4* base = reinterpret_cast<const uint4*>(row - shift * E::kSize);
-  const int vectors = (V + shift + kVec - 1) / kVec;
-  const int v0 = static_cast<int>(static_cast<int64_t>(vectors) * part / parts);
-  const int v1 = static_cast<int>(static_cast<int64_t>(vectors) * (part + 1) / parts);
-  const int inner0 = shift ? 1 : 0, inner1 = (V + shift) / kVec;  // whole vectors
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  const int V = a.vocab, top = a.top, rows_at_once = gridDim.x / parts;
+  const auto part_of = [&](int r) {
+    Part p;
+    p.row = static_cast<const char*>(a.logits) + r * a.stride * E::kSize;
+    p.shift = static_cast<int>(reinterpret_cast<uintptr_t>(p.row) & 15) / E::kSize;
+    p.base = reinterpret_cast<const uint4*>(p.row - p.shift * E::kSize);
+    const int vectors = (V + p.shift + kVec - 1) / kVec;
+    p.v0 = static_cast<int>(static_cast<int64_t>(vectors) * part / parts);
+    p.v1 = static_cast<int>(static_cast<int64_t>(vectors) * (part + 1) / parts);
+    p.inner0 = p.shift ? 1 : 0;
+    p.inner1 = (V + p.shift) / kVec;
+    return p;
+  };
   uint4* ring = reinterpret_cast<uint4*>(dynamic) + t;  // (stage, vector) at ring[(stage * kU + u) * kT]
-  const auto fill = [&](int stage, int v) {  // the batch that starts with vector v
+  const auto fill = [&](const Part& p, int stage, int v) {  // the batch that starts with vector v
 #pragma unroll
-    for (int u = 0; u < kU && v < v1; ++u) {
+    for (int u = 0; u < kU && v < p.v1; ++u) {
       uint4* dst = ring + (stage * kU + u) * kT;
       const int w = v + u * kT;
-      if (w >= inner0 && w < min(inner1, v1))
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(base + w) : "memory");
+      if (w >= p.inner0 && w < min(p.inner1, p.v1))
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(p.base + w) : "memory");
       else
-        *dst = w < v1 ? edge_vector<DT>(row, w * kVec - shift, V) : make_uint4(E::kNegInf, E::kNegInf, E::kNegInf, E::kNegInf);
+        *dst = w < p.v1 ? edge_vector<DT>(p.row, w * kVec - p.shift, V)
+                        : make_uint4(E::kNegInf, E::kNegInf, E::kNegInf, E::kNegInf);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-
-  // ---- the pass
-  Sums mine{-INFINITY, 0.f, 0.f};
-  float seg = -INFINITY, best = -INFINITY;
-  int in_seg = 0, n_seg = 0;
-  uint64_t l2 = 0, s2 = 0;
+  // the first batches of a part, to be read from `stage` on
+  const auto start = [&](const Part& p, int stage) {
 #pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) fill(i, v0 + t + i * kU * kT);
+    for (int i = 0; i < kStages - 1; ++i) fill(p, (stage + i) % kStages, p.v0 + t + i * kU * kT);
+  };
   int stage = 0;
-  for (int v = v0 + t; v < v1; v += kU * kT) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-    uint4 x[kU];
-#pragma unroll
-    for (int u = 0; u < kU; ++u) x[u] = ring[(stage * kU + u) * kT];
-    fill(stage == 0 ? kStages - 1 : stage - 1, v + (kStages - 1) * kU * kT);
-    stage = stage == kStages - 1 ? 0 : stage + 1;
-    uint32_t m = x[0].x;
-#pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      m = E::larger(m, E::larger(x[u].x, x[u].y));
-      m = E::larger(m, E::larger(x[u].z, x[u].w));
-    }
-    const float big = E::value(m);
-    if (big > mine.ref + kHeadroom) {
-      float p, q;
-      unpack_f32x2(l2, p, q);
-      mine.l = p + q;
-      unpack_f32x2(s2, p, q);
-      mine.s = p + q;
-      mine.move(big);
-      l2 = pack_f32x2(mine.l, 0.f);
-      s2 = pack_f32x2(mine.s, 0.f);
-    }
-    seg = max_nan(seg, big);
-    if (top > 0 && ++in_seg == per_segment) {
-      segs[n_seg++ * kT + t] = seg;
-      best = max_nan(best, seg);
-      seg = -INFINITY;
-      in_seg = 0;
-    }
-    const float ref = mine.ref == -INFINITY ? 0.f : mine.ref;
-    const uint64_t nref = pack_f32x2(-ref, -ref), scale = pack_f32x2(kLog2e, kLog2e);
-    const auto two = [&](float x0, float x1) {
-      const uint64_t y = fmul2(fadd2(pack_f32x2(x0, x1), nref), scale);
-      float y0, y1;
-      unpack_f32x2(y, y0, y1);
-      const uint64_t e = pack_f32x2(ex2(y0), ex2(y1));
-      l2 = fadd2(l2, e);
-      // e is 0 where the clamp acts (-inf logits)
-      s2 = ffma2(e, pack_f32x2(fmaxf(y0, -1000.f), fmaxf(y1, -1000.f)), s2);
-    };
-#pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
-      if constexpr (DT == 2) {
-        two(__uint_as_float(w[0]), __uint_as_float(w[1]));
-        two(__uint_as_float(w[2]), __uint_as_float(w[3]));
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 f = E::pair(w[i]);
-          two(f.x, f.y);
-        }
-      }
-    }
-  }
-  {
-    float p, q;
-    unpack_f32x2(l2, p, q);
-    mine.l = p + q;
-    unpack_f32x2(s2, p, q);
-    mine.s = p + q;
-  }
-#pragma unroll
-  for (int s = 16; s > 0; s /= 2)
-    mine = joined(mine, Sums{__shfl_xor_sync(0xffffffffu, mine.ref, s), __shfl_xor_sync(0xffffffffu, mine.l, s),
-                             __shfl_xor_sync(0xffffffffu, mine.s, s)});
-  if (lane == 0) sh.warp_sums[warp] = mine;
+  Part next = part_of(blockIdx.x / parts);
+  start(next, stage);
+  for (int r = blockIdx.x / parts; r < a.rows; r += rows_at_once) {
+    const Part p = next;
 
-  // ---- this part's alternatives
-  const int have = min(V, v1 * kVec - shift) - max(0, v0 * kVec - shift);  // its elements
-  const int k = min(top, max(have, 0));
-  if (k > 0) {
-    if (in_seg > 0) {
-      segs[n_seg++ * kT + t] = seg;
-      best = max_nan(best, seg);
+    // thread 0 has the token's logit long before its sums
+    int64_t token = -1;
+    float token_logit = 0.f;
+    if (part == 0 && t == 0) {
+      token = a.tokens[r];
+      if (token >= 0 && token < V) token_logit = E::at(p.row, token);
     }
-    // the k-th largest of the maxima of 2 k or more groups of lanes (32, 64 or 128 groups)
-    const int lanes = k <= 16 ? kT / 32 : k <= 32 ? kT / 64 : 1;  // of a group
-    float g = best;
-    for (int s = 1; s < lanes; s *= 2) g = max_nan(g, __shfl_xor_sync(0xffffffffu, g, s));
-    const uint32_t group_key = value_key(g);
-    if (t % lanes == 0) reinterpret_cast<uint32_t*>(sh.groups)[t / lanes] = group_key;
-    if (t == 0) {
-      sh.count = 0;
-      sh.hits = 0;
-      sh.bound = 0;
-    }
-    asm volatile("cp.async.wait_all;" ::: "memory");  // the ring's place is free
-    __syncthreads();
-    if (t < kT / lanes) {
-      const uint32_t key = reinterpret_cast<const uint32_t*>(sh.groups)[t];
-      int above = 0;
-#pragma unroll 4
-      for (int i = 0; i < kT / lanes / 4; ++i) {
-        const uint4 o = sh.groups[i];
-        above += (o.x > key || (o.x == key && 4 * i < t)) + (o.y > key || (o.y == key && 4 * i + 1 < t)) +
-                 (o.z > key || (o.z == key && 4 * i + 2 < t)) + (o.w > key || (o.w == key && 4 * i + 3 < t));
+
+    // ---- the pass
+    Sums mine{-INFINITY, 0.f, 0.f};
+    float seg = -INFINITY, best = -INFINITY;
+    int in_seg = 0, n_seg = 0;
+    uint64_t l2 = 0, s2 = 0;
+    for (int v = p.v0 + t; v < p.v1; v += kU * kT) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+      uint4 x[kU];
+#pragma unroll
+      for (int u = 0; u < kU; ++u) x[u] = ring[(stage * kU + u) * kT];
+      fill(p, stage == 0 ? kStages - 1 : stage - 1, v + (kStages - 1) * kU * kT);
+      stage = stage == kStages - 1 ? 0 : stage + 1;
+      uint32_t m = x[0].x;
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        m = E::larger(m, E::larger(x[u].x, x[u].y));
+        m = E::larger(m, E::larger(x[u].z, x[u].w));
       }
-      if (above == k - 1) sh.bound = key;
-    }
-    __syncthreads();
-    // candidates: every value at or above the bound; `strict`: above it.  The
-    // segments that reach it are listed first; then a warp reads one at a time.
-    const auto collect = [&](uint32_t bound, bool strict) {
-      for (int i = 0; i < n_seg; ++i) {
-        const uint32_t sk = value_key(segs[i * kT + t]);
-        if (strict ? sk > bound : sk >= bound) hit_list[atomicAdd(&sh.hits, 1)] = static_cast<uint16_t>(i * kT + t);
+      const float big = E::value(m);
+      if (big > mine.ref + kHeadroom) {
+        float x0, x1;
+        unpack_f32x2(l2, x0, x1);
+        mine.l = x0 + x1;
+        unpack_f32x2(s2, x0, x1);
+        mine.s = x0 + x1;
+        mine.move(big);
+        l2 = pack_f32x2(mine.l, 0.f);
+        s2 = pack_f32x2(mine.s, 0.f);
       }
-      __syncthreads();
-      const int hits = sh.hits, each = per_segment * kU * kVec;
-      for (int i = warp; i < hits; i += kT / 32) {
-        const int hit = hit_list[i], first = v0 + hit % kT + hit / kT * per_segment * kU * kT;
-#pragma unroll 1
-        for (int j = lane; j < each; j += 32) {
-          const int v = first + j / kVec * kT, e = v * kVec - shift + j % kVec;
-          if (v >= v1 || e < 0 || e >= V) continue;
-          const float y = E::at(row, e);
-          const uint32_t key = value_key(y);
-          if (strict ? key <= bound : key < bound) continue;
-          const int at = atomicAdd(&sh.count, 1);
-          if (at < kCandidates) cand[at] = rank_key(y, e);
+      seg = max_nan(seg, big);
+      if (top > 0 && ++in_seg == per_segment) {
+        segs[n_seg++ * kT + t] = seg;
+        best = max_nan(best, seg);
+        seg = -INFINITY;
+        in_seg = 0;
+      }
+      const float ref = mine.ref == -INFINITY ? 0.f : mine.ref;
+      const uint64_t nref = pack_f32x2(-ref, -ref), scale = pack_f32x2(kLog2e, kLog2e);
+      const auto two = [&](float x0, float x1) {
+        const uint64_t y = fmul2(fadd2(pack_f32x2(x0, x1), nref), scale);
+        float y0, y1;
+        unpack_f32x2(y, y0, y1);
+        const uint64_t e = pack_f32x2(ex2(y0), ex2(y1));
+        l2 = fadd2(l2, e);
+        // e is 0 where the clamp acts (-inf logits)
+        s2 = ffma2(e, pack_f32x2(fmaxf(y0, -1000.f), fmaxf(y1, -1000.f)), s2);
+      };
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        const uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+        if constexpr (DT == 2) {
+          two(__uint_as_float(w[0]), __uint_as_float(w[1]));
+          two(__uint_as_float(w[2]), __uint_as_float(w[3]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = E::pair(w[i]);
+            two(f.x, f.y);
+          }
         }
       }
+    }
+    if (r + rows_at_once < a.rows) {
+      next = part_of(r + rows_at_once);
+      start(next, stage);
+    }
+    {
+      float x0, x1;
+      unpack_f32x2(l2, x0, x1);
+      mine.l = x0 + x1;
+      unpack_f32x2(s2, x0, x1);
+      mine.s = x0 + x1;
+    }
+    {
+      float to = mine.ref;
+#pragma unroll
+      for (int s = 16; s > 0; s /= 2) to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, s));
+      mine.move(to == -INFINITY ? 0.f : to);
+      mine.ref = to;
+#pragma unroll
+      for (int s = 16; s > 0; s /= 2) {
+        mine.l += __shfl_xor_sync(0xffffffffu, mine.l, s);
+        mine.s += __shfl_xor_sync(0xffffffffu, mine.s, s);
+      }
+    }
+    if (lane == 0) sh.warp_sums[warp] = mine;
+
+    // ---- this part's alternatives
+    const int have = min(V, p.v1 * kVec - p.shift) - max(0, p.v0 * kVec - p.shift);  // its elements
+    const int k = min(top, max(have, 0));
+    if (k > 0) {
+      if (in_seg > 0) {
+        segs[n_seg++ * kT + t] = seg;
+        best = max_nan(best, seg);
+      }
+      // the k-th largest of the maxima of 2 k or more groups of lanes (32, 64 or 128 groups)
+      const int lanes = k <= 16 ? kT / 32 : k <= 32 ? kT / 64 : 1;  // of a group
+      float g = best;
+      for (int s = 1; s < lanes; s *= 2) g = max_nan(g, __shfl_xor_sync(0xffffffffu, g, s));
+      const uint32_t group_key = value_key(g);
+      if (t % lanes == 0) reinterpret_cast<uint32_t*>(sh.groups)[t / lanes] = group_key;
+      if (t == 0) {
+        sh.count = 0;
+        sh.hits = 0;
+        sh.bound = 0;
+      }
       __syncthreads();
-    };
-    uint32_t bound = sh.bound;
-    collect(bound, false);
-    int n = sh.count;
-    __syncthreads();
-    // Too many: the values above the bound alone.  Are these too many as well,
-    // the k-th largest of those at hand is a higher bound.
-    while (n > kCandidates) {
-      if (t == 0) sh.count = sh.hits = 0;
+      if (t < kT / lanes) {
+        const uint32_t key = reinterpret_cast<const uint32_t*>(sh.groups)[t];
+        int above = 0;
+#pragma unroll 4
+        for (int i = 0; i < kT / lanes / 4; ++i) {
+          const uint4 o = sh.groups[i];
+          above += (o.x > key || (o.x == key && 4 * i < t)) + (o.y > key || (o.y == key && 4 * i + 1 < t)) +
+                   (o.z > key || (o.z == key && 4 * i + 2 < t)) + (o.w > key || (o.w == key && 4 * i + 3 < t));
+        }
+        if (above == k - 1) sh.bound = key;
+      }
       __syncthreads();
-      collect(bound, true);
-      n = sh.count;
+      // candidates: every value at or above the bound; `strict`: above it.  The
+      // segments that reach it are listed first; then their elements are read again.
+      // (Most segments at the bound are most of the row at one value, such as
+      // logits masked to -inf: too many without a look.)
+      const auto collect = [&](uint32_t bound, bool strict) {
+        for (int i = 0; i < n_seg; ++i) {
+          const uint32_t sk = value_key(segs[i * kT + t]);
+          if (strict ? sk > bound : sk >= bound) hit_list[atomicAdd(&sh.hits, 1)] = static_cast<uint16_t>(i * kT + t);
+        }
+        __syncthreads();
+        const int hits = sh.hits, each = per_segment * kU * kVec;
+        if (!strict && hits > kManyHits && have > kCandidates) return kCandidates + 1;
+        // (eight loads of a thread in flight: the row may have left L2)
+        for (int i = t; i < hits * each; i += kLook * kT) {
+          float y[kLook];
+          int at[kLook];
+#pragma unroll
+          for (int u = 0; u < kLook; ++u) {
+            const int q = i + u * kT, hit = hit_list[min(q / each, hits - 1)], j = q % each;
+            const int v = p.v0 + hit % kT + (hit / kT * per_segment * kU + j / kVec) * kT;
+            at[u] = q < hits * each && v < p.v1 ? v * kVec - p.shift + j % kVec : -1;
+            if (at[u] >= V) at[u] = -1;
+            y[u] = at[u] >= 0 ? E::at(p.row, at[u]) : 0.f;
+          }
+#pragma unroll
+          for (int u = 0; u < kLook; ++u) {
+            const uint32_t key = value_key(y[u]);
+            if (at[u] < 0 || (strict ? key <= bound : key < bound)) continue;
+            const int to = atomicAdd(&sh.count, 1);
+            if (to < kCandidates) cand[to] = rank_key(y[u], at[u]);
+          }
+        }
+        __syncthreads();
+        return sh.count;
+      };
+      uint32_t bound = sh.bound;
+      int n = collect(bound, false);
       __syncthreads();
-      if (n > kCandidates) {
-        select_top(cand, kCandidates, k, sh.best, sh);
-        bound = static_cast<uint32_t>(sh.best[k - 1] >> 32);
+      // Too many: the values above the bound alone.  Are these too many as well,
+      // the k-th largest of those at hand is a higher bound.
+      while (n > kCandidates) {
         if (t == 0) sh.count = sh.hits = 0;
         __syncthreads();
-        collect(bound, false);
-        n = sh.count;
+        n = collect(bound, true);
         __syncthreads();
-      } else if (n < k) {
-        // the lowest indices among the values equal to the bound
-        const int e0 = max(0, v0 * kVec - shift), e1 = min(V, v1 * kVec - shift);
-        int need = k - n;
-        for (int e = e0; e < e1 && need > 0; e += kT) {
-          const bool tie = e + t < e1 && value_key(E::at(row, e + t)) == bound;
-          const uint32_t votes = __ballot_sync(0xffffffffu, tie);
-          if (lane == 0) sh.votes[warp] = __popc(votes);
+        if (n > kCandidates) {
+          select_top(cand, kCandidates, k, sh.best);
+          bound = static_cast<uint32_t>(sh.best[k - 1] >> 32);
+          if (t == 0) sh.count = sh.hits = 0;
           __syncthreads();
-          int before = __popc(votes & ((1u << lane) - 1)), all = 0;
-          for (int w = 0; w < kT / 32; ++w) {
-            if (w < warp) before += sh.votes[w];
-            all += sh.votes[w];
+          n = collect(bound, false);
+          __syncthreads();
+        } else if (n < k) {
+          // the lowest indices among the values equal to the bound
+          const int e0 = max(0, p.v0 * kVec - p.shift), e1 = min(V, p.v1 * kVec - p.shift);
+          int need = k - n;
+          for (int e = e0; e < e1 && need > 0; e += kT) {
+            const bool tie = e + t < e1 && value_key(E::at(p.row, e + t)) == bound;
+            const uint32_t votes = __ballot_sync(0xffffffffu, tie);
+            if (lane == 0) sh.votes[warp] = __popc(votes);
+            __syncthreads();
+            int before = __popc(votes & ((1u << lane) - 1)), all = 0;
+            for (int w = 0; w < kT / 32; ++w) {
+              if (w < warp) before += sh.votes[w];
+              all += sh.votes[w];
+            }
+            if (tie && before < need) cand[n + before] = rank_key(key_value(bound), e + t);
+            n += min(all, need);
+            need -= min(all, need);
+            __syncthreads();
           }
-          if (tie && before < need) cand[n + before] = rank_key(key_value(bound), e + t);
-          n += min(all, need);
-          need -= min(all, need);
-          __syncthreads();
         }
       }
+      select_top(cand, n, k, sh.best);
     }
-    select_top(cand, n, k, sh.best, sh);
-  }
-  __syncthreads();
-  if (t == 0) {
-    Sums all = sh.warp_sums[0];
-    for (int w = 1; w < kT / 32; ++w) all = joined(all, sh.warp_sums[w]);
-    sh.sums = all;
-    sh.picked = k;
-  }
-
-  // ---- the parts joined by the cluster's first CTA
-  if (parts > 1) {
-    cluster.sync();
-    if (part == 0 && top > 0) {
-      int n = 0;
-      for (int i = 0; i < parts; ++i) {
-        const Shared* other = cluster.map_shared_rank(&sh, i);
-        const int m = other->picked;
-        for (int j = t; j < m; j += kT) sh.merged[n + j] = other->best[j];
-        n += m;
-      }
-      __syncthreads();
-      select_top(sh.merged, n, top, sh.best, sh);
-    }
-  } else {
     __syncthreads();
-  }
-  if (part == 0) {
-    Sums all = sh.sums;
-    for (int i = 1; i < parts; ++i) all = joined(all, cluster.map_shared_rank(&sh, i)->sums);
-    const bool nothing = all.l == 0.f;  // every logit -inf
-    const float ref = all.ref == -INFINITY ? 0.f : all.ref, logl = logf(all.l);
     if (t == 0) {
-      const int64_t token = a.tokens[r];
-      float lp = 0.f;
-      if (token >= V) {
-        atomicCAS(a.status, 0, kStatusBadToken);
-        lp = __int_as_float(0x7fc00000);
-      } else if (token >= 0) {
-        lp = nothing ? -INFINITY : (E::at(row, token) - ref) - logl;
+      Sums all = sh.warp_sums[0];
+      for (int w = 1; w < kT / 32; ++w) all = joined(all, sh.warp_sums[w]);
+      sh.sums = all;
+      sh.picked = k;
+    }
+
+    // ---- the parts joined by the cluster's first CTA
+    if (parts > 1) {
+      cluster.sync();
+      if (part == 0 && top > 0) {
+        int n = 0;
+        for (int i = 0; i < parts; ++i) {
+          const Shared* other = cluster.map_shared_rank(&sh, i);
+          const int m = other->picked;
+          for (int j = t; j < m; j += kT) sh.merged[n + j] = other->best[j];
+          n += m;
+        }
+        __syncthreads();
+        select_top(sh.merged, n, top, sh.best);
       }
-      a.logprobs[r] = lp;
-      a.entropy[r] = nothing ? 0.f : logl - kLn2 * (all.s / all.l);
+    } else {
+      __syncthreads();
     }
-    for (int i = t; i < top; i += kT) {
-      const uint64_t key = sh.best[i];
-      a.top_ids[static_cast<int64_t>(r) * top + i] = 0xffffffffu - static_cast<uint32_t>(key);
-      a.top_logprobs[static_cast<int64_t>(r) * top + i] =
-          nothing ? -INFINITY : (key_value(static_cast<uint32_t>(key >> 32)) - ref) - logl;
+    if (part == 0) {
+      Sums all = sh.sums;
+      for (int i = 1; i < parts; ++i) all = joined(all, cluster.map_shared_rank(&sh, i)->sums);
+      const bool nothing = all.l == 0.f;  // every logit -inf
+      const float ref = all.ref == -INFINITY ? 0.f : all.ref, logl = logf(all.l);
+      if (t == 0) {
+        float lp = 0.f;
+        if (token >= V) {
+          atomicCAS(a.status, 0, kStatusBadToken);
+          lp = __int_as_float(0x7fc00000);
+        } else if (token >= 0) {
+          lp = nothing ? -INFINITY : (token_logit - ref) - logl;
+        }
+        a.logprobs[r] = lp;
+        a.entropy[r] = nothing ? 0.f : logl - kLn2 * (all.s / all.l);
+      }
+      for (int i = t; i < top; i += kT) {
+        const uint64_t key = sh.best[i];
+        a.top_ids[static_cast<int64_t>(r) * top + i] = 0xffffffffu - static_cast<uint32_t>(key);
+        a.top_logprobs[static_cast<int64_t>(r) * top + i] =
+            nothing ? -INFINITY : (key_value(static_cast<uint32_t>(key >> 32)) - ref) - logl;
+      }
     }
+    if (parts > 1) cluster.sync();  // the others' shared memory is read until here
+    else __syncthreads();           // as this CTA's own is
   }
-  if (parts > 1) cluster.sync();  // the others' shared memory is read until here
 }
 
 template <int DT>
 cudaError_t launch(const ScoreArgs& a, cudaStream_t st) {
-  // CTAs of a row: while the GPU holds all of them at once (six an SM) and each has two vectors a
-  // thread.
+  // CTAs of a row: while the GPU holds all of them at once and each has two vectors a thread.
   constexpr int kVec = Type<DT>::kVec;
   const int64_t vectors = static_cast<int64_t>(a.vocab) / kVec + 2;
   int parts = 1;
-  while (parts < kMaxCluster && static_cast<int64_t>(a.rows) * parts * 2 <= 148 * 6 &&
+  while (parts < kMaxCluster && static_cast<int64_t>(a.rows) * parts * 2 <= kSms * kResident &&
          vectors / (parts * 2) >= 2 * kT)
     parts *= 2;
   const int64_t batches = (vectors / parts + 1 + kU * kT - 1) / (kU * kT);  // of a thread
   const int per_segment = static_cast<int>((batches + kSegments - 1) / kSegments);
   const int64_t segments = (batches + per_segment - 1) / per_segment;
-  const size_t smem = kRing + (a.top > 0 ? static_cast<size_t>(segments) * kT * 4 : 0);
-  if (static_cast<int64_t>(a.rows) * parts > 0x7FFFFFFF) return cudaErrorInvalidValue;
+  const size_t smem = kRing + (a.top > 0 ? kCandidates * 8 + static_cast<size_t>(segments) * kT * 4 : 0);
+  const int rows = a.rows < kSms * kResident ? a.rows : kSms * kResident;  // at once
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(a.rows) * parts);
+  cfg.gridDim = dim3(static_cast<unsigned>(rows) * parts);
   cfg.blockDim = dim3(kT);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
