@@ -341,7 +341,9 @@ int rp_paged_append(const rp_paged_kv* kv, const void* k_new, const void* v_new,
                     const int32_t* lengths, int B, float* weights, const int64_t* weight_strides,
                     int64_t weight_cols, int32_t* lengths_out, void* stream);
 
-/* Workspace bytes rp_paged_decode needs. */
+/* Workspace bytes rp_paged_decode needs: a few MB that depend on head_dim and
+ * Hq / heads, and with weights 4 bytes per query head and position that the
+ * page tables can address. */
 int rp_paged_decode_workspace_bytes(const rp_paged_kv* kv, int B, int Hq, int table_pages,
                                     int with_weights, size_t* bytes);
 

@@ -25,7 +25,8 @@ constexpr int kAppendThreads = 256;
 // and each lane then divides for one of the 2 U scales.  Reads 4 D bytes and
 // writes 2 D (or 4 D) a row: HBM bounds it, and the instruction rate is near
 // (254 instructions a thread and row before the sharing, and 71 % of all issue
-// slots).
+// slots).  Measured: 48 prompts of 512 to 4099 tokens, 8 heads of 128, into an
+// e4m3 cache 139 us, 5.1 TB/s; one token of 64 sequences 2.8 us.
 template <int D, bool E4M3, bool F16, int U>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs a) {
   constexpr int kLanes = D / 8;                     // threads a row
@@ -165,8 +166,9 @@ cudaError_t append_u(const AppendArgs& a, cudaStream_t st) {
   return cudaGetLastError();
 }
 
-// Two rows a thread once the GPU is full all the same (148 SMs of 2048 threads): 48 prompts of 8
-// heads took 172 us with one row, 139 with two, 145 with four, 192 with eight.
+// Two rows a thread once the GPU is full all the same (148 SMs of 2048 threads):
+// the 48 prompts took 139 us with two, 145 with four (and, with every row's
+// reductions and divisions its own, 172 with one and 192 with eight).
 template <int D>
 cudaError_t append_d(const AppendArgs& a, cudaStream_t st) {
   const int64_t threads = static_cast<int64_t>(a.tokens) * a.kv.heads * (D / 8);
@@ -199,7 +201,8 @@ __device__ __forceinline__ float key_weight(uint32_t k) {
 // matching of lanes that avoids them, take most of the time.)  Two passes more
 // count and place what is kept in order, so ties at the threshold go to the
 // lowest positions.  Reads each weight from HBM once; bound by the latency of
-// its few dependent passes, which the split over a cluster shortens.
+// its few dependent passes, which the split over a cluster shortens.  Measured:
+// 16 rows of 70001 and 98303 weights 27 us, 128 rows of 1001 to 16385 25 us.
 constexpr int kSelThreads = 256;
 constexpr int kSelWarps = kSelThreads / 32;
 static_assert(kSelThreads >= 256, "a thread for every sum of 8 bins");
@@ -426,7 +429,9 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
 // ---- move
 //
 // Kept rows to their new places: a warp takes 8 rows, their places found by 8
-// lanes, with K and V of all of them in flight before the first store.
+// lanes, with K and V of all of them in flight before the first store.  Bound by
+// HBM: 4096 rows of 128 sequences and heads (bf16, D 128) 85 us, 6.1 TB/s read
+// and written.
 constexpr int kMoveRows = 8;
 constexpr int kMoveWarps = 8;
 

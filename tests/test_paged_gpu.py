@@ -233,6 +233,17 @@ def test_decode_splits_long_and_few_rows(kv, lengths):
     assert torch.equal(out, again) and torch.equal(lse, lse2) and torch.equal(first, weights)
 
 
+@pytest.mark.parametrize("kv", ["fp16", "e4m3"])
+def test_decode_many_sequences(kv):
+    """More sequences than a CTA has threads, many of them empty."""
+    lengths = [(37 * i) % 211 if i % 3 else 0 for i in range(700)]
+    cache, table, n, _, _ = filled(lengths, 1, 16, 64, kv, seed=6)
+    q = rows((700, 4, 64), torch.float16 if kv == "fp16" else torch.bfloat16, 14)
+    check_decode(q, cache, table, n, torch.zeros((700, 1, table.shape[1] * 16), device="cuda"))
+    empty = torch.zeros_like(n)
+    check_decode(q, cache, table, empty)
+
+
 def test_decode_wide_table_strides_streams_and_scale():
     """A page table far wider than the sequences, q and out inside packed
     tensors, a table with padded rows, a scale of the caller's, another stream."""
@@ -393,6 +404,22 @@ def test_evict_selects_exactly_in_long_sequences(n, budget, recent):
     got = paged.evict(cache, table, torch.tensor([n], dtype=torch.int32, device="cuda"), w, out_table, budget=budget, recent=recent)
     for h in range(H):
         assert got.kept[0, h].tolist() == op.kept_positions(w[0, h].cpu().numpy(), n, budget, recent).tolist()
+
+
+@pytest.mark.parametrize("heads, width, n, budget", [(1, 6000, 750000, 5000), (256, 360, 3000, 700)])
+def test_evict_without_room_for_the_keys_on_chip(heads, width, n, budget):
+    """Page tables so wide that a CTA's slice of the weights does not fit shared
+    memory: few rows (16 CTAs each) and many (one CTA each)."""
+    from repercep_runtime_b200 import paged
+
+    page = 128
+    table, pages = make_table([n], page, width)
+    out_table, extra = make_table([budget], page, first=pages)
+    cache = paged.alloc(pages + extra, heads, page, 32, torch.float8_e4m3fn)
+    w = accumulated((1, heads, width * page), 13)
+    got = paged.evict(cache, table, torch.tensor([n], dtype=torch.int32, device="cuda"), w, out_table, budget=budget, recent=9)
+    for h in range(0, heads, 51):
+        assert got.kept[0, h].tolist() == op.kept_positions(w[0, h].cpu().numpy(), n, budget, 9).tolist()
 
 
 # ---------------------------------------------------------------- refusals
