@@ -15,21 +15,22 @@ namespace cg = cooperative_groups;
 constexpr int kAppendThreads = 256;
 
 // New rows into the cache.  A row of D 16-bit values is D / 8 16-byte
-// vectors, one a thread, so a warp holds 256 / D rows; a CTA takes a run of U *
-// 2048 / D rows, numbered (token, head) as the input has them.  While the K and
+// vectors; a thread takes one, or for an e4m3 cache two, so that it stores 16
+// bytes of K and of V each time (8 took 139 us where 16 take 115).  A CTA takes
+// a run of rows, numbered (token, head) as the input has them.  While the K and
 // V vectors of a thread's U rows are on their way, one thread per token finds
 // its sequence, page and slot (done by every thread for every row, this took
 // twice the time of the rest).  e4m3: the steps are the quantizer's
 // (quant_common.cuh), so the bytes are those of the row-wise quantizer; K's and
-// V's amax share the words of one shuffle reduction over the row's D / 8 lanes,
+// V's amax share the words of one shuffle reduction over the row's D / 16 lanes,
 // and each lane then divides for one of the 2 U scales.  Reads 4 D bytes and
-// writes 2 D (or 4 D) a row: HBM bounds it, and the instruction rate is near
-// (254 instructions a thread and row before the sharing, and 71 % of all issue
-// slots).  Measured: 48 prompts of 512 to 4099 tokens, 8 heads of 128, into an
-// e4m3 cache 139 us, 5.1 TB/s; one token of 64 sequences 2.8 us.
+// writes 2 D (or 4 D) a row, bound by HBM.  Measured: 48 prompts of 512 to 4099
+// tokens, 8 heads of 128, into an e4m3 cache 115 us, 6.2 TB/s; one token of 64
+// sequences 2.8 us.
 template <int D, bool E4M3, bool F16, int U>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs a) {
-  constexpr int kLanes = D / 8;                     // threads a row
+  constexpr int kVecs = E4M3 ? 2 : 1;               // 16-byte vectors of a thread: it writes 16 bytes of K and of V
+  constexpr int kLanes = D / 8 / kVecs;             // threads a row
   constexpr int kAtOnce = kAppendThreads / kLanes;  // rows a CTA takes at once
   constexpr int kTokens = kAtOnce * U;              // tokens of a CTA, at most
   __shared__ int64_t offset[kTokens];               // of (token, head 0), -1: left out
@@ -40,7 +41,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
   const uint32_t rows = static_cast<uint32_t>(a.tokens) * H, begin = blockIdx.x * kTokens;
   const uint32_t r0 = begin + threadIdx.x / kLanes;
   const uint32_t next_tok = kAtOnce / H, next_head = kAtOnce % H;
-  uint4 k[U], v[U];
+  uint4 k[U][kVecs], v[U][kVecs];
   uint32_t tok[U], head[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -51,10 +52,13 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
       head[u] -= H;
       ++tok[u];
     }
-    k[u] = v[u] = make_uint4(0, 0, 0, 0);
-    if (r < rows) {
-      k[u] = __ldcs(reinterpret_cast<const uint4*>(a.k_new + tok[u] * a.k_tok + head[u] * a.k_head) + c);
-      v[u] = __ldcs(reinterpret_cast<const uint4*>(a.v_new + tok[u] * a.v_tok + head[u] * a.v_head) + c);
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      k[u][i] = v[u][i] = make_uint4(0, 0, 0, 0);
+      if (r < rows) {
+        k[u][i] = __ldg(reinterpret_cast<const uint4*>(a.k_new + tok[u] * a.k_tok + head[u] * a.k_head) + c * kVecs + i);
+        v[u][i] = __ldg(reinterpret_cast<const uint4*>(a.v_new + tok[u] * a.v_tok + head[u] * a.v_head) + c * kVecs + i);
+      }
     }
   }
   for (uint32_t i = blockIdx.x * kAppendThreads + threadIdx.x; i < B; i += gridDim.x * kAppendThreads) {
@@ -105,7 +109,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
     uint32_t m[U];  // amax bits: K's in the low half, V's in the high one
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      m[u] = quant::absmax8(k[u]) | quant::absmax8(v[u]) << 16;
+      m[u] = max(quant::absmax8(k[u][0]), quant::absmax8(k[u][1])) |
+             max(quant::absmax8(v[u][0]), quant::absmax8(v[u][1])) << 16;
 #pragma unroll
       for (int x = kLanes / 2; x > 0; x /= 2) m[u] = __vmaxu2(m[u], __shfl_xor_sync(0xffffffffu, m[u], x));
     }
@@ -135,15 +140,17 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
       const float qv = __shfl_sync(0xffffffffu, mul[(2 * u + 1) / kLanes], (2 * u + 1) % kLanes, kLanes);
       if (off[u] < 0) continue;
       // a scale that is inf or NaN has a reciprocal that is not positive
-      reinterpret_cast<uint2*>(a.kv.k + off[u])[c] = quant::quant8_any<F16>(k[u], qk, qk > 0.f);
-      reinterpret_cast<uint2*>(a.kv.v + off[u])[c] = quant::quant8_any<F16>(v[u], qv, qv > 0.f);
+      const uint2 k0 = quant::quant8_any<F16>(k[u][0], qk, qk > 0.f), k1 = quant::quant8_any<F16>(k[u][1], qk, qk > 0.f);
+      const uint2 v0 = quant::quant8_any<F16>(v[u][0], qv, qv > 0.f), v1 = quant::quant8_any<F16>(v[u][1], qv, qv > 0.f);
+      reinterpret_cast<uint4*>(a.kv.k + off[u])[c] = make_uint4(k0.x, k0.y, k1.x, k1.y);
+      reinterpret_cast<uint4*>(a.kv.v + off[u])[c] = make_uint4(v0.x, v0.y, v1.x, v1.y);
     }
   } else {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (off[u] < 0) continue;
-      reinterpret_cast<uint4*>(a.kv.k + 2 * off[u])[c] = k[u];
-      reinterpret_cast<uint4*>(a.kv.v + 2 * off[u])[c] = v[u];
+      reinterpret_cast<uint4*>(a.kv.k + 2 * off[u])[c] = k[u][0];
+      reinterpret_cast<uint4*>(a.kv.v + 2 * off[u])[c] = v[u][0];
     }
   }
   if (a.weights.w && c == 0) {
@@ -155,7 +162,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
 
 template <int D, int U>
 cudaError_t append_u(const AppendArgs& a, cudaStream_t st) {
-  constexpr int kRows = kAppendThreads / (D / 8) * U;  // of a CTA
+  const int kRows = kAppendThreads / (D / 8) * (a.kv.dtype == kKvE4m3 ? 2 : 1) * U;  // of a CTA
   const int64_t rows = static_cast<int64_t>(a.tokens) * a.kv.heads;
   int64_t grid = (rows + kRows - 1) / kRows;
   if (grid < 1) grid = 1;  // lengths_out
@@ -167,8 +174,7 @@ cudaError_t append_u(const AppendArgs& a, cudaStream_t st) {
 }
 
 // Two rows a thread once the GPU is full all the same (148 SMs of 2048 threads):
-// the 48 prompts took 139 us with two, 145 with four (and, with every row's
-// reductions and divisions its own, 172 with one and 192 with eight).
+// the 48 prompts take 115 us with two, 132 with one, 145 with four.
 template <int D>
 cudaError_t append_d(const AppendArgs& a, cudaStream_t st) {
   const int64_t threads = static_cast<int64_t>(a.tokens) * a.kv.heads * (D / 8);

@@ -96,13 +96,21 @@ class PagedKV:
         s = k.stride()
         strides = s[:3] if bhsd else (s[0], s[2], s[1])
         object.__setattr__(self, "_geometry", (strides, _KV[k.dtype], self.num_pages, self.heads, self.page_size, D))
+        object.__setattr__(self, "_kv", _lib.PagedKVStruct(*self._pointers(), *self._geometry))
 
-    def _struct(self) -> _lib.PagedKVStruct:
+    def _pointers(self) -> tuple[int | None, ...]:
         ks, vs = self.k_scales, self.v_scales
-        return _lib.PagedKVStruct(
+        return (
             self.k.data_ptr(), self.v.data_ptr(),
-            None if ks is None else ks.data_ptr(), None if vs is None else vs.data_ptr(), *self._geometry,
+            None if ks is None else ks.data_ptr(), None if vs is None else vs.data_ptr(),
         )  # fmt: skip
+
+    def _struct(self):  # type: ignore[no-untyped-def]
+        """A pointer to ``rp_paged_kv`` of the tensors as they are now."""
+        kv, now = self._kv, self._pointers()
+        if (kv.k, kv.v, kv.k_scales, kv.v_scales) != now:  # a tensor was given another storage
+            kv = _lib.PagedKVStruct(*now, *self._geometry)
+        return byref(kv)
 
 
 def alloc(
@@ -205,7 +213,7 @@ def append(
     w, w_strides, w_cols = _weights(cache, weights, B, pages)
     out = torch.empty_like(lengths)
     _lib.launch(
-        device.index, "rp_paged_append", byref(cache._struct()), k_new.data_ptr(), v_new.data_ptr(),
+        device.index, "rp_paged_append", cache._struct(), k_new.data_ptr(), v_new.data_ptr(),
         _I64x4(k0, k1, v0, v1), _HALF[dtype], tokens, None if starts is None else starts.data_ptr(),
         page_table.data_ptr(), row, pages, lengths.data_ptr(), B, w, w_strides, w_cols, out.data_ptr(),
     )  # fmt: skip
@@ -262,18 +270,18 @@ def decode(
     if scale is not None and not 0.0 < scale < float("inf"):
         raise ValueError(f"scale must be positive and finite, got {scale}")
     if out is None:
-        out = q.new_empty(shape)
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
     elif out.shape != shape or out.dtype != dtype or out.device != device or out.stride(2) != 1:
         raise ValueError("out must have q's shape, dtype and device, with a unit-stride head dim")
     o0, o1, _ = out.stride()
     if (B > 1 and o0 == 0) or (Hq > 1 and o1 == 0):
         raise ValueError("rows of out overlap")
-    lse = torch.empty((B, Hq), dtype=torch.float32, device=device) if return_lse else None
+    lse = q.new_empty((B, Hq), dtype=torch.float32) if return_lse else None
     w, w_strides, w_cols = _weights(cache, weights, B, pages)
     need = _decode_workspace(cache._geometry, B, Hq, pages, weights is not None)
     ws = torch.empty(need, dtype=torch.uint8, device=device)
     _lib.launch(
-        device.index, "rp_paged_decode", byref(cache._struct()), q.data_ptr(), _I64x2(q0, q1), _HALF[dtype], B, Hq,
+        device.index, "rp_paged_decode", cache._struct(), q.data_ptr(), _I64x2(q0, q1), _HALF[dtype], B, Hq,
         page_table.data_ptr(), row, pages, lengths.data_ptr(), 0.0 if scale is None else float(scale),
         out.data_ptr(), _I64x2(o0, o1), None if lse is None else lse.data_ptr(), w, w_strides, w_cols,
         ws.data_ptr(), need,
@@ -325,7 +333,7 @@ def evict(
     new_lengths = torch.empty_like(lengths)
     new_weights = torch.empty((B, cache.heads, out_pages * cache.page_size), dtype=torch.float32, device=device)
     _lib.launch(
-        device.index, "rp_paged_evict", byref(cache._struct()), page_table.data_ptr(), row, pages, lengths.data_ptr(), B,
+        device.index, "rp_paged_evict", cache._struct(), page_table.data_ptr(), row, pages, lengths.data_ptr(), B,
         w, w_strides, w_cols, out_table.data_ptr(), out_row, out_pages, budget, recent,
         kept.data_ptr(), new_lengths.data_ptr(), new_weights.data_ptr(),
     )  # fmt: skip
