@@ -329,9 +329,9 @@ def evict(
     if weights is None:
         raise ValueError("evict needs the accumulated weights")
     w, w_strides, w_cols = _weights(cache, weights, B, pages)
-    kept = torch.empty((B, cache.heads, budget), dtype=torch.int32, device=device)
+    kept = lengths.new_empty((B, cache.heads, budget))
     new_lengths = torch.empty_like(lengths)
-    new_weights = torch.empty((B, cache.heads, out_pages * cache.page_size), dtype=torch.float32, device=device)
+    new_weights = weights.new_empty((B, cache.heads, out_pages * cache.page_size))
     _lib.launch(
         device.index, "rp_paged_evict", cache._struct(), page_table.data_ptr(), row, pages, lengths.data_ptr(), B,
         w, w_strides, w_cols, out_table.data_ptr(), out_row, out_pages, budget, recent,

@@ -61,10 +61,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
     top = int(top)
     if not 0 <= top <= min(MAX_TOP, vocab):
         raise ValueError(f"top must be in [0, {min(MAX_TOP, vocab)}], got {top}")
-    logprobs = torch.empty(rows, dtype=torch.float32, device=device)
+    logprobs = logits.new_empty(rows, dtype=torch.float32)
     entropy = torch.empty_like(logprobs)
-    top_logprobs = torch.empty((rows, top), dtype=torch.float32, device=device)
-    top_ids = torch.empty((rows, top), dtype=torch.int64, device=device)
+    top_logprobs = logprobs.new_empty((rows, top))
+    top_ids = tokens.new_empty((rows, top))
     args = (
         logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, _LOGITS[logits.dtype], rows, vocab,
         tokens.data_ptr(), top, logprobs.data_ptr(), entropy.data_ptr(), top_logprobs.data_ptr(), top_ids.data_ptr(),
