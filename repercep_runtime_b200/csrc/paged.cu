@@ -202,9 +202,9 @@ __device__ __forceinline__ float key_weight(uint32_t k) {
 // key) is found in at most three passes over them, 11, 11 and 10 bits at a
 // time, with a histogram per CTA that every CTA of the cluster adds up through
 // distributed shared memory: sums of 8 bins first, then the bins of one such
-// sum.  (All 2048 bins at once take 4500 cycles a pass; 8 bits at a time do not
-// work either: weights share few exponents, and the adds to a few bins, or the
-// matching of lanes that avoids them, take most of the time.)  Two passes more
+// sum.  (All 2048 bins at once take 4500 cycles a pass; counting the lanes of a
+// bin by ballots or a match before one add costs more than the adds, also where
+// weights are equal: 57 us against 52 for two long sequences.)  Two passes more
 // count and place what is kept in order, so ties at the threshold go to the
 // lowest positions.  Reads each weight from HBM once; bound by the latency of
 // its few dependent passes, which the split over a cluster shortens.  Measured:
@@ -293,13 +293,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
       }
 #pragma unroll
       for (int u = 0; u < kSelBatch; ++u) {
-        // lanes of the first such lane's bin are counted by one add: rows with many equal weights
-        const uint32_t live = __ballot_sync(0xffffffffu, in[u]);
-        if (live == 0) continue;
-        const int bin = (key[u] >> shift) & ((1 << bits) - 1), lead = __ffs(live) - 1;
-        const int bin0 = __shfl_sync(0xffffffffu, bin, lead);
-        const uint32_t same = __ballot_sync(0xffffffffu, in[u] && bin == bin0);
-        if (in[u] && (bin != bin0 || lane == lead)) atomicAdd(&hist[bin], bin == bin0 ? __popc(same) : 1);
+        if (in[u]) atomicAdd(&hist[(key[u] >> shift) & ((1 << bits) - 1)], 1);
       }
     }
     __syncthreads();
