@@ -31,10 +31,10 @@
 //    remainder, two products each, which cost 1 % of the time; rounded once it
 //    added as much error as the output's own rounding (2.2e-3 against 1.7e-3 in
 //    all).  With an e4m3 cache it is rounded once, to fp16 (relative 2^-11).
-// Measured, main kernel: two sequences of 115k tokens, 32/8 heads, fp16 146 us
-// (6.8 TB/s); 64 sequences of 512 to 520, 32/32 heads, bf16, with scores kept for
-// the weights 86 us (6.3 TB/s); 128 of 1 to 8191, 32/8 heads, e4m3, with scores
-// 200 us (5.8 TB/s, the scores' writes included).  The join takes 5 us, the
+// Measured, main kernel: two sequences of 115k tokens, 32/8 heads, fp16 144 us
+// (6.9 TB/s); 64 sequences of 512 to 520, 32/32 heads, bf16, with scores kept for
+// the weights 84 us (6.5 TB/s); 128 of 1 to 8191, 32/8 heads, e4m3, with scores
+// 196 us (5.9 TB/s, the scores' writes included).  The join takes 5 us, the
 // weights of that last batch 20 us (their traffic).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
