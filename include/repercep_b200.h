@@ -305,8 +305,9 @@ int rp_quant_fp8_rows(const void* x, int64_t ldx, int in_dtype, int rows, int co
  * What only the device can see is checked there: a page id outside the pool
  * (0x201), a length below 0 or past the page table (0x202) and a token id
  * past the vocabulary (0x203) are recorded in the device status word and
- * never read or written through: such a row is skipped, such a length is cut
- * to the nearest valid one. */
+ * never read or written through: such a row is skipped, such a length is read
+ * as the nearest valid one (but a negative one takes no new token, see
+ * rp_paged_append). */
 typedef enum rp_kv_dtype {
   RP_KV_BF16 = 0,
   RP_KV_F16 = 1,
@@ -334,7 +335,8 @@ typedef struct rp_paged_kv {
  *   weights       NULL or accumulated attention weights (B, heads,
  *                 weight_cols) at b * weight_strides[0] + h *
  *                 weight_strides[1] + p: zeroed at the new positions
- *   lengths_out   (B) lengths after the call; not the memory of lengths */
+ *   lengths_out   (B) lengths after the call; not the memory of lengths.  A
+ *                 sequence of negative length takes no token and keeps it */
 int rp_paged_append(const rp_paged_kv* kv, const void* k_new, const void* v_new,
                     const int64_t* new_strides, int in_dtype, int tokens, const int32_t* starts,
                     const int32_t* page_table, int64_t table_stride, int table_pages,

@@ -64,7 +64,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
   for (uint32_t i = blockIdx.x * kAppendThreads + threadIdx.x; i < B; i += gridDim.x * kAppendThreads) {
     const int n = table_length(a.t, a.kv.page_size, i, a.status);
     const int64_t add = a.starts ? static_cast<int64_t>(a.starts[i + 1]) - a.starts[i] : 1;
-    a.lengths_out[i] = static_cast<int>(n + (add > 0 ? add : 0));
+    // a negative length takes no token and stays: as a 0, the next call's would go over position 0
+    a.lengths_out[i] = a.t.lengths[i] < 0 ? a.t.lengths[i] : static_cast<int>(n + (add > 0 ? add : 0));
   }
   const uint32_t t0 = begin / H, t1 = (min(begin + kTokens, rows) + H - 1) / H;  // the run's tokens
   for (uint32_t i = threadIdx.x; begin < rows && i < t1 - t0; i += kAppendThreads) {
@@ -84,8 +85,9 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
     }
     int64_t off = -1;
     if (ok) {
-      const int64_t pos = static_cast<int64_t>(table_length(a.t, a.kv.page_size, b, a.status)) + (t - first);
-      if (pos < 0 || pos >= static_cast<int64_t>(a.t.pages) * a.kv.page_size) {
+      const int n = a.t.lengths[b];
+      const int64_t pos = static_cast<int64_t>(n) + (t - first);
+      if (n < 0 || pos < 0 || pos >= static_cast<int64_t>(a.t.pages) * a.kv.page_size) {
         atomicCAS(a.status, 0, kStatusBadLength);
       } else {
         const int p = static_cast<int>(pos);

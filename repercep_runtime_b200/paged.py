@@ -15,9 +15,11 @@ is one pool of pages that sequences take as they grow and may share:
 
 Position p of sequence b is slot ``p % page_size`` of page ``page_table[b, p //
 page_size]``.  Tables and lengths are int32 CUDA tensors and stay on the device
-(no call synchronises); entries past a sequence's pages are not read.  A page
-id, length or token position that does not fit is skipped on the device and
-recorded in its status word (``_lib.device_status``).
+(no call synchronises); entries past a sequence's pages are not read.  What
+does not fit is recorded in the device's status word (``_lib.device_status``):
+a row whose page id is outside the pool and a new token past the page table are
+skipped, a length is read as the nearest valid one, and a sequence of negative
+length takes no new token.
 
 Torch allocates outputs and workspaces and supplies the current stream; the
 arithmetic runs in the library, which has no fallback (a missing library
@@ -190,7 +192,8 @@ def append(
     sequence (tokens outside [starts[0], starts[-1]) are left out); without it
     every sequence gets one token.  An e4m3 cache takes each row's scale and
     bytes from ``linear.quantize_rows``'s recipe.  ``weights`` are zeroed at
-    the new positions."""
+    the new positions.  A sequence of negative length takes nothing and keeps
+    that length."""
     device, dtype = cache.device, k_new.dtype
     B, pages, row = _table(device, "page_table", page_table)
     _lengths(device, lengths, B)

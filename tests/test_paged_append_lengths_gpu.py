@@ -1,0 +1,59 @@
+"""Appends whose lengths do not fit, on the GPU: what is written, what is left
+alone, the lengths that come back and the device status."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+from test_paged_gpu import DTYPES, filled, rows
+
+pytestmark = pytest.mark.gpu
+
+BAD_LENGTH = 0x202
+
+
+def status() -> int:
+    from repercep_runtime_b200 import _lib
+
+    return _lib.device_status(reset=True)
+
+
+@pytest.fixture(autouse=True)
+def healthy():
+    status()
+    yield
+    assert status() == 0
+
+
+def pools(cache):
+    """The bytes of every tensor of a cache."""
+    names = ("k", "v") + (("k_scales", "v_scales") if cache.k_scales is not None else ())
+    return {x: getattr(cache, x).view(torch.uint8).clone() for x in names}
+
+
+@pytest.mark.parametrize("kv, half", [("bf16", "bf16"), ("e4m3", "fp16")])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_a_negative_length_takes_no_token(kv, half, ragged):
+    """Nothing of that sequence is written, and its length stays as it is: a
+    length of 0 in its place would let the next call write over position 0."""
+    from repercep_runtime_b200 import paged
+
+    cache, table, n, _, _ = filled([20, 20, 20], 2, 16, 64, kv, half=DTYPES[half], seed=1)
+    n[0], n[2] = -1, -2
+    before = pools(cache)
+    counts = [2, 3, 1] if ragged else [1, 1, 1]
+    starts = torch.tensor([0] + counts).cumsum(0).to(torch.int32).cuda() if ragged else None
+    new = rows((sum(counts), 2, 64), DTYPES[half], 2)
+    weights = torch.full((3, 2, table.shape[1] * 16), 7.0, device="cuda")
+    got = paged.append(cache, new, new, table, n, starts=starts, weights=weights)
+    assert status() == BAD_LENGTH
+    assert got.tolist() == [-1, 20 + counts[1], -2]
+    assert bool((weights[[0, 2]] == 7).all())
+    after = pools(cache)
+    page = int(table[1, 1])  # where sequence 1 took its tokens, from slot 4 on
+    for name, x in after.items():
+        unit = 4 if "scales" in name else 1  # bytes of a scale lie in the slots' dimension
+        taken = (page, slice(None), slice(4 * unit, (4 + counts[1]) * unit))
+        assert not torch.equal(x[taken], before[name][taken])
+        x[taken] = before[name][taken]
+        assert torch.equal(x, before[name]), name
