@@ -335,8 +335,9 @@ typedef struct rp_paged_kv {
  *   weights       NULL or accumulated attention weights (B, heads,
  *                 weight_cols) at b * weight_strides[0] + h *
  *                 weight_strides[1] + p: zeroed at the new positions
- *   lengths_out   (B) lengths after the call; not the memory of lengths.  A
- *                 sequence of negative length takes no token and keeps it */
+ *   lengths_out   (B) lengths after the call, at most what the page table can
+ *                 address; not the memory of lengths.  A sequence of negative
+ *                 length takes no token and keeps it */
 int rp_paged_append(const rp_paged_kv* kv, const void* k_new, const void* v_new,
                     const int64_t* new_strides, int in_dtype, int tokens, const int32_t* starts,
                     const int32_t* page_table, int64_t table_stride, int table_pages,

@@ -64,8 +64,10 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
   for (uint32_t i = blockIdx.x * kAppendThreads + threadIdx.x; i < B; i += gridDim.x * kAppendThreads) {
     const int n = table_length(a.t, a.kv.page_size, i, a.status);
     const int64_t add = a.starts ? static_cast<int64_t>(a.starts[i + 1]) - a.starts[i] : 1;
-    // a negative length takes no token and stays: as a 0, the next call's would go over position 0
-    a.lengths_out[i] = a.t.lengths[i] < 0 ? a.t.lengths[i] : static_cast<int>(n + (add > 0 ? add : 0));
+    // what the table holds is counted; a negative length takes no token and stays: as a 0, the
+    // next call's would go over position 0
+    const int64_t after = min(n + (add > 0 ? add : 0), static_cast<int64_t>(a.t.pages) * a.kv.page_size);
+    a.lengths_out[i] = a.t.lengths[i] < 0 ? a.t.lengths[i] : static_cast<int>(after);
   }
   const uint32_t t0 = begin / H, t1 = (min(begin + kTokens, rows) + H - 1) / H;  // the run's tokens
   for (uint32_t i = threadIdx.x; begin < rows && i < t1 - t0; i += kAppendThreads) {

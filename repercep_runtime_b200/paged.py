@@ -192,8 +192,8 @@ def append(
     sequence (tokens outside [starts[0], starts[-1]) are left out); without it
     every sequence gets one token.  An e4m3 cache takes each row's scale and
     bytes from ``linear.quantize_rows``'s recipe.  ``weights`` are zeroed at
-    the new positions.  A sequence of negative length takes nothing and keeps
-    that length."""
+    the new positions.  Tokens past the page table are not counted; a sequence
+    of negative length takes nothing and keeps that length."""
     device, dtype = cache.device, k_new.dtype
     B, pages, row = _table(device, "page_table", page_table)
     _lengths(device, lengths, B)

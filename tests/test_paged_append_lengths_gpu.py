@@ -5,7 +5,7 @@ from __future__ import annotations
 
 import pytest
 import torch
-from test_paged_gpu import DTYPES, filled, rows
+from test_paged_gpu import DTYPES, filled, heads_first, rows
 
 pytestmark = pytest.mark.gpu
 
@@ -57,3 +57,29 @@ def test_a_negative_length_takes_no_token(kv, half, ragged):
         assert not torch.equal(x[taken], before[name][taken])
         x[taken] = before[name][taken]
         assert torch.equal(x, before[name]), name
+
+
+@pytest.mark.parametrize("kv", ["fp16", "e4m3"])
+def test_lengths_stop_at_the_end_of_the_table(kv):
+    """Tokens that fit are stored, and the lengths count these alone, so that
+    the calls after it have lengths that fit."""
+    from repercep_runtime_b200 import paged
+
+    cache, table, n, _, _ = filled([48, 48, 48, 48, 48], 1, 16, 64, kv, half=torch.float16, seed=3)
+    n = torch.tensor([46, 48, 60, 10, 2**31 - 2], dtype=torch.int32, device="cuda")
+    starts = torch.tensor([0, 3, 6, 9, 12, 15], dtype=torch.int32, device="cuda")
+    new = rows((15, 1, 64), torch.float16, 4)
+    before = pools(cache)
+    got = paged.append(cache, new, new, table, n, starts=starts)
+    assert status() == BAD_LENGTH
+    assert got.tolist() == [48, 48, 48, 13, 48]
+    changed = torch.zeros((cache.num_pages, 16), dtype=torch.bool, device="cuda")
+    for b, p in [(0, 46), (0, 47), (3, 10), (3, 11), (3, 12)]:
+        changed[table[b, p // 16].long(), p % 16] = True
+    differs = (heads_first(cache, cache.k).contiguous().view(torch.uint8) != before["k"].view(cache.num_pages, 1, 16, -1)).any(-1)[:, 0]
+    assert torch.equal(differs, changed)
+    paged.decode(rows((5, 1, 64), torch.float16, 5), cache, table, got)
+    assert status() == 0
+    # one token each
+    got = paged.append(cache, new[:5], new[:5], table, torch.tensor([47, 48, 49, 0, 2**31 - 1], dtype=torch.int32, device="cuda"))
+    assert status() == BAD_LENGTH and got.tolist() == [48, 48, 48, 1, 48]
