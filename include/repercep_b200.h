@@ -303,8 +303,9 @@ int rp_quant_fp8_rows(const void* x, int64_t ldx, int in_dtype, int rows, int co
  *              rows, contiguous (num_pages, heads, page_size)
  * head_dim in {32, 64, 128, 256}; any page_size.
  * What only the device can see is checked there: a page id outside the pool
- * (0x201), a length below 0 or past the page table (0x202) and a token id
- * past the vocabulary (0x203) are recorded in the device status word and
+ * (0x201), a length below 0 or past the page table or starts that descend or
+ * lie outside the new tokens (0x202) and a token id past the vocabulary
+ * (0x203) are recorded in the device status word and
  * never read or written through: such a row is skipped, such a length is read
  * as the nearest valid one (but a negative one takes no new token, see
  * rp_paged_append). */
@@ -331,7 +332,8 @@ typedef struct rp_paged_kv {
  *   starts        (B + 1) int32 first new token of each sequence: token t of
  *                 starts[b] <= t < starts[b + 1] goes to position lengths[b]
  *                 + t - starts[b]; tokens outside [starts[0], starts[B]) are
- *                 left out.  NULL: token b is sequence b's one new token
+ *                 left out, and starts outside [0, tokens] count as its
+ *                 ends.  NULL: token b is sequence b's one new token
  *   weights       NULL or accumulated attention weights (B, heads,
  *                 weight_cols) at b * weight_strides[0] + h *
  *                 weight_strides[1] + p: zeroed at the new positions

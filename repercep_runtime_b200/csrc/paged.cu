@@ -63,10 +63,15 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
   }
   for (uint32_t i = blockIdx.x * kAppendThreads + threadIdx.x; i < B; i += gridDim.x * kAppendThreads) {
     const int n = table_length(a.t, a.kv.page_size, i, a.status);
-    const int64_t add = a.starts ? static_cast<int64_t>(a.starts[i + 1]) - a.starts[i] : 1;
+    int add = 1;
+    if (a.starts) {  // the tokens of it that there are
+      const int s0 = a.starts[i], s1 = a.starts[i + 1];
+      if (s0 < 0 || s1 < s0 || s1 > a.tokens) atomicCAS(a.status, 0, kStatusBadLength);
+      add = max(0, min(max(s1, 0), a.tokens) - max(s0, 0));
+    }
     // what the table holds is counted; a negative length takes no token and stays: as a 0, the
     // next call's would go over position 0
-    const int64_t after = min(n + (add > 0 ? add : 0), static_cast<int64_t>(a.t.pages) * a.kv.page_size);
+    const int64_t after = min(static_cast<int64_t>(n) + add, static_cast<int64_t>(a.t.pages) * a.kv.page_size);
     a.lengths_out[i] = a.t.lengths[i] < 0 ? a.t.lengths[i] : static_cast<int>(after);
   }
   const uint32_t t0 = begin / H, t1 = (min(begin + kTokens, rows) + H - 1) / H;  // the run's tokens
@@ -83,13 +88,13 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
         else hi = mid - 1;
       }
       b = lo;
-      first = __ldg(a.starts + b);
+      first = max(0, __ldg(a.starts + b));
     }
     int64_t off = -1;
     if (ok) {
       const int n = a.t.lengths[b];
       const int64_t pos = static_cast<int64_t>(n) + (t - first);
-      if (n < 0 || pos < 0 || pos >= static_cast<int64_t>(a.t.pages) * a.kv.page_size) {
+      if (n < 0 || pos >= static_cast<int64_t>(a.t.pages) * a.kv.page_size) {
         atomicCAS(a.status, 0, kStatusBadLength);
       } else {
         const int p = static_cast<int>(pos);

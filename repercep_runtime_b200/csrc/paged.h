@@ -10,7 +10,7 @@ namespace rp {
 
 // Codes these kernels record in the device status word.
 constexpr int kStatusBadPage = 0x201;    // a page id outside the pool
-constexpr int kStatusBadLength = 0x202;  // a length below 0 or past the page table
+constexpr int kStatusBadLength = 0x202;  // a length below 0 or past the page table, bad starts
 constexpr int kStatusBadToken = 0x203;   // a token id past the vocabulary
 
 // Value types of a cache (rp_kv_dtype).

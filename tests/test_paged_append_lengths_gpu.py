@@ -1,5 +1,5 @@
-"""Appends whose lengths do not fit, on the GPU: what is written, what is left
-alone, the lengths that come back and the device status."""
+"""Appends whose lengths or starts do not fit, on the GPU: what is written, what
+is left alone, the lengths that come back and the device status."""
 
 from __future__ import annotations
 
@@ -83,3 +83,29 @@ def test_lengths_stop_at_the_end_of_the_table(kv):
     # one token each
     got = paged.append(cache, new[:5], new[:5], table, torch.tensor([47, 48, 49, 0, 2**31 - 1], dtype=torch.int32, device="cuda"))
     assert status() == BAD_LENGTH and got.tolist() == [48, 48, 48, 1, 48]
+
+
+def test_starts_outside_the_new_tokens_count_what_is_there():
+    """Lengths grow by the tokens that were given, and a sequence's first one
+    goes right behind its length."""
+    from repercep_runtime_b200 import paged
+
+    new = rows((4, 2, 64), torch.bfloat16, 6)
+    for starts, counts, first in [([0, 2, 9], [2, 2], [0, 2]), ([-3, 2, 4], [2, 2], [0, 2]), ([0, 7, 9], [4, 0], [0, 4])]:
+        cache, table, n, _, _ = filled([20, 25], 2, 16, 64, "bf16", width=2, seed=7)
+        got = paged.append(cache, new, new, table, n, starts=torch.tensor(starts, dtype=torch.int32, device="cuda"))
+        assert status() == BAD_LENGTH, starts
+        assert got.tolist() == [20 + counts[0], 25 + counts[1]], starts
+        for b, (length, count, at) in enumerate(zip((20, 25), counts, first)):
+            for i in range(count):
+                p = length + i
+                assert torch.equal(cache.k[int(table[b, p // 16]), :, p % 16], new[at + i]), (starts, b, i)
+
+
+def test_descending_starts_are_reported():
+    from repercep_runtime_b200 import paged
+
+    cache, table, n, _, _ = filled([3, 4, 5], 2, 16, 64, "bf16", seed=8)
+    new = rows((6, 2, 64), torch.bfloat16, 9)
+    got = paged.append(cache, new, new, table, n, starts=torch.tensor([0, 4, 2, 6], dtype=torch.int32, device="cuda"))
+    assert status() == BAD_LENGTH and got.tolist()[1] == 4
