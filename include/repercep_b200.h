@@ -300,7 +300,10 @@ int rp_quant_fp8_rows(const void* x, int64_t ldx, int in_dtype, int rows, int co
  *              strides[1] + slot * strides[2]) elements, head_dim elements
  *              of dtype (one set of strides for both; 16-byte multiples)
  *   k_scales, v_scales   RP_KV_E4M3 only: fp32 dequant multipliers of the
- *              rows, contiguous (num_pages, heads, page_size)
+ *              rows, contiguous (num_pages, heads, page_size).  A row whose
+ *              scale is 0 is zeros, whatever its bytes: the quantizer's fp16
+ *              scale of an fp16 row below 1.27e-5 rounds to 0, and the bytes
+ *              of that row's zeros are NaN
  * head_dim in {32, 64, 128, 256}; any page_size.
  * What only the device can see is checked there: a page id outside the pool
  * (0x201), a length below 0 or past the page table or starts that descend or

@@ -70,3 +70,34 @@ def token_scores(x: np.ndarray, token: int, top: int) -> dict[str, object]:
         p = e / total
         entropy = -np.where(p == 0, 0.0, p * np.where(p == 0, 0.0, logp)).sum()
     return dict(logprob=0.0 if token < 0 else logp[token], entropy=entropy, ids=order, top=logp[order])
+
+
+def decode_bound(
+    q: np.ndarray, k: np.ndarray, v: np.ndarray, scale: float, out_round: float, weight_round: float, floor: np.ndarray
+) -> dict[str, np.ndarray]:
+    """Bounds on the rounding errors of one sequence's decode, element by element.
+
+    Scores are fp32 sums of exact products: e_j = D 2^-23 scale sum_d |q_d k_jd|
+    + 2^-20 bounds key j's (the constant also takes exp and log in fp32), and
+    e = sum_j p_j e_j the log-sum-exp's.  The sums over keys take fp32 steps of
+    16 keys in 4 or more chains, two products a step: n / 32 + 8 steps, each off
+    by 2^-21 of what it adds to.  A weight is rounded by ``weight_round`` of
+    itself, or by ``floor`` (Hq, n) in units of the exact weights where that is
+    more; the output once by ``out_round``.
+
+    ``out`` (Hq, D), ``lse`` (Hq,)."""
+    ref = decode(q, k, v, scale)
+    Hq, D = q.shape
+    H, n = k.shape[0], k.shape[1]
+    if n == 0:
+        return dict(out=np.zeros((Hq, D)), lse=np.zeros(Hq))
+    g = q.reshape(H, Hq // H, D)
+    s = np.einsum("hgd,hnd->hgn", g, k) * scale
+    p = np.exp(s - s.max(-1, keepdims=True))
+    p /= p.sum(-1, keepdims=True)
+    e = D * 2.0**-23 * abs(scale) * np.einsum("hgd,hnd->hgn", np.abs(g), np.abs(k)) + 2.0**-20
+    e_lse = (p * e).sum(-1)
+    chain = (n / 32 + 8) * 2.0**-21
+    each = p * (weight_round + 2 * e + 2 * e_lse[..., None] + 2 * chain) + floor.reshape(H, Hq // H, n)
+    out = np.einsum("hgn,hnd->hgd", each, np.abs(v)).reshape(Hq, D) * (1 + out_round)
+    return dict(out=out + out_round * np.abs(ref["out"]), lse=2 * e_lse.reshape(Hq) + chain + 2.0**-21 * np.abs(ref["lse"]))

@@ -25,7 +25,9 @@
 //  - e4m3 rows are widened to fp16 exactly.  The queries are brought to fp16
 //    by a power of two of their row's maximum, the rows' K scales multiply the
 //    scores in fp32, and their V scales the softmax weights, over a running
-//    power of two that keeps those within fp16's range.
+//    power of two that keeps those within fp16's range.  A row whose scale is 0
+//    (fp16 rows of zeros or below 1.27e-5, whose scale the quantizer rounds to 0
+//    and whose zeros are NaN bytes) is cleared in shared memory first.
 //  - Rounding: scores, sums and accumulators are fp32.  For the product with a
 //    16-bit V a softmax weight is split into a 16-bit value and the 16-bit
 //    remainder, two products each, which cost 1 % of the time; rounded once it
@@ -450,6 +452,22 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
         const auto chunk = [&](uint32_t base, int r, int col) {
           return base + r * C::kRow + ((col ^ ((r >> kRsh) & kMask)) << 4);
         };
+        uint8_t* rows = smem + warp * C::kRing + stage * C::kStage;
+        const float* scales = reinterpret_cast<const float*>(rows + 2 * C::kRowsBytes);
+        if constexpr (C::kFp8) {
+          // a row whose scale is 0 is zeros, whatever its bytes (0 times a NaN byte is not)
+          const uint32_t k0 = __ballot_sync(0xffffffffu, scales[my_key] == 0.f) & mask;
+          const uint32_t v0 = __ballot_sync(0xffffffffu, scales[C::kKeys + my_key] == 0.f) & mask;
+          if (k0 | v0) {
+#pragma unroll 1
+            for (int r = 0; r < C::kKeys; ++r) {
+              uint4* dst = reinterpret_cast<uint4*>(rows + r * C::kRow) + lane;
+              if (((k0 >> r) & 1) && lane < C::kChunks) *dst = make_uint4(0, 0, 0, 0);
+              if (((v0 >> r) & 1) && lane < C::kChunks) dst[C::kRowsBytes / 16] = make_uint4(0, 0, 0, 0);
+            }
+            __syncwarp();
+          }
+        }
         // ---- S^T = K Q^T
         float x[MT][NT][4];
 #pragma unroll
@@ -486,8 +504,6 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
           }
         }
         // ---- scores in log2 units; what is not live is -inf
-        const float* scales = reinterpret_cast<const float*>(smem + warp * C::kRing + stage * C::kStage +
-                                                             2 * C::kRowsBytes);
         float top[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) top[nt][0] = top[nt][1] = -INFINITY;

@@ -50,8 +50,9 @@ class PagedKV:
     """A pool of pages: ``k`` and ``v`` (pages, heads, page_size, D) for layout
     "bhsd" (a page in the place of a batch), (pages, page_size, heads, D) for
     "bshd"; bf16, fp16, or e4m3 with fp32 ``k_scales`` / ``v_scales`` (pages,
-    heads, page_size), one dequant multiplier per row.  D is unit-stride and k
-    and v share their strides."""
+    heads, page_size), one dequant multiplier per row; a row whose scale is 0 is
+    zeros, whatever its bytes (``append`` leaves such a row for fp16 values all
+    below 1.27e-5).  D is unit-stride and k and v share their strides."""
 
     k: torch.Tensor
     v: torch.Tensor
