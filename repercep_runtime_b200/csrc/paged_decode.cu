@@ -24,15 +24,19 @@
 //    pipe's cycles; tcgen05's 128 rows would meet the same few queries.
 //  - e4m3 rows are widened to fp16 exactly.  The queries are brought to fp16
 //    by a power of two of their row's maximum, the rows' K scales multiply the
-//    scores in fp32, and their V scales the softmax weights, over a running
-//    power of two that keeps those within fp16's range.  A row whose scale is 0
+//    scores in fp32, and their V scales the softmax weights.  The products of
+//    weight and V scale enter fp16 over a running power of two of their own
+//    maximum in each column (over the largest V scale alone, a large row of no
+//    weight pushed the others' out of fp16's range).  A row whose scale is 0
 //    (fp16 rows of zeros or below 1.27e-5, whose scale the quantizer rounds to 0
 //    and whose zeros are NaN bytes) is cleared in shared memory first.
 //  - Rounding: scores, sums and accumulators are fp32.  For the product with a
 //    16-bit V a softmax weight is split into a 16-bit value and the 16-bit
 //    remainder, two products each, which cost 1 % of the time; rounded once it
 //    added as much error as the output's own rounding (2.2e-3 against 1.7e-3 in
-//    all).  With an e4m3 cache it is rounded once, to fp16 (relative 2^-11).
+//    all).  With an e4m3 cache it is rounded once, with its V scale, to fp16:
+//    relative 2^-11, and absolutely 2^-35 of the column's largest such product
+//    (two parts there cost 2 to 10 %: 233 us for the batch below, 73 for 16 heads).
 // Measured, main kernel: two sequences of 115k tokens, 32/8 heads, fp16 144 us
 // (6.9 TB/s); 64 sequences of 512 to 520, 32/32 heads, bf16, with scores kept for
 // the weights 84 us (6.5 TB/s); 128 of 1 to 8191, 32/8 heads, e4m3, with scores
@@ -57,9 +61,11 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kJoinThreads = 512;
 constexpr int kMaxCtas = 592;  // CTAs of the main kernel, at most
 constexpr int kMinTiles = 2;    // tiles of a CTA's run, at least (but for the last)
-// The running maximum of a row is raised only when a score exceeds it by this
-// much (log2 units): until then 2^(s - m) <= 256, and nothing is rescaled.
-constexpr float kRescale = 8.f;
+// e4m3: a weight times its row's V scale enters fp16 times a power of two of its
+// column's, which brings the largest such product to 2^10 or more, falls when one
+// exceeds 2^15, and is at most 2^110.
+constexpr float kWeightTop = 32768.f;
+constexpr uint32_t kWeightMost = 127 + 110;
 
 template <int KV, int D, int NT>
 struct Cfg {
@@ -68,6 +74,10 @@ struct Cfg {
   static constexpr int kRow = D * (kFp8 ? 1 : 2);   // bytes of a row
   static constexpr int kChunks = kRow / 16;         // 16-byte chunks of a row
   static constexpr int kFrags = D / 16 * NT;  // accumulator fragments (float4 a lane)
+  // The reference m of a row's weights 2^(s - m) (log2 units): a new one lies kBelow
+  // under the maximum, and stays until a score exceeds it by kAbove.  e4m3: weights
+  // are at most 1, so that a product with any V scale is finite.
+  static constexpr float kBelow = kFp8 ? -8.f : 0.f, kAbove = kBelow + 8.f;
   // keys of a warp's step: 16 where that makes 8 KB (a stage holds a warp's accumulators at times)
   static constexpr int kKeys = 32 * kRow >= 8192 && 32 * kRow >= kFrags * 512 ? 16 : 32;
   static constexpr int kTile = kKeys * kWarps;
@@ -428,9 +438,11 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
       }
     }
 
-    float m[NT][2], l[NT][2], o[DT][NT][4], vref = __uint_as_float(27u << 23);  // 2^-100
+    float m[NT][2], l[NT][2], o[DT][NT][4];
+    float winv[NT][2];  // e4m3: the power of two by which weights with their V scales enter fp16
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+      winv[nt][0] = winv[nt][1] = __uint_as_float(kWeightMost << 23);
       m[nt][0] = m[nt][1] = -INFINITY;
       l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
@@ -456,9 +468,9 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
         const float* scales = reinterpret_cast<const float*>(rows + 2 * C::kRowsBytes);
         if constexpr (C::kFp8) {
           // a row whose scale is 0 is zeros, whatever its bytes (0 times a NaN byte is not)
-          const uint32_t k0 = __ballot_sync(0xffffffffu, scales[my_key] == 0.f) & mask;
-          const uint32_t v0 = __ballot_sync(0xffffffffu, scales[C::kKeys + my_key] == 0.f) & mask;
-          if (k0 | v0) {
+          const bool no_k = scales[my_key] == 0.f, no_v = scales[C::kKeys + my_key] == 0.f;
+          if (__any_sync(0xffffffffu, (no_k || no_v) && ((mask >> my_key) & 1))) {
+            const uint32_t k0 = __ballot_sync(0xffffffffu, no_k), v0 = __ballot_sync(0xffffffffu, no_v);
 #pragma unroll 1
             for (int r = 0; r < C::kKeys; ++r) {
               uint4* dst = reinterpret_cast<uint4*>(rows + r * C::kRow) + lane;
@@ -547,7 +559,7 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) raise |= top[nt][j] > m[nt][j] + kRescale;
+          for (int j = 0; j < 2; ++j) raise |= top[nt][j] > m[nt][j] + C::kAbove;
         if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
@@ -557,7 +569,7 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
               t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
               t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
               t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
-              t = fmaxf(t, m[nt][j]);
+              t = fmaxf(t - C::kBelow, m[nt][j]);
               const float f = t == m[nt][j] ? 1.f : ex2(m[nt][j] - t);
               m[nt][j] = t;
               l[nt][j] *= f;
@@ -568,23 +580,54 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
               }
             }
         }
-        float vinv = 1.f;
         if constexpr (C::kFp8) {
-          uint32_t v = __float_as_uint(scales[C::kKeys + my_key]) & 0x7fffffffu;
-          v = __reduce_max_sync(0xffffffffu, v);
-          if (v > __float_as_uint(vref)) {
-            // the next power of two, at most 2^126 (a scale above it is inf, NaN or as good as)
-            const float ref = __uint_as_float(min((v + 0x7fffffu) & 0x7f800000u, 253u << 23));
-            const float f = vref / ref;
-            vref = ref;
+          // weights with their rows' V scales, and their maximum in each column
+          float top_w[NT][2];
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
+          for (int nt = 0; nt < NT; ++nt) top_w[nt][0] = top_w[nt][1] = 0.f;
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float vs = scales[C::kKeys + mt * 16 + i * 8 + row];
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[dt][nt][i] *= f;
+                for (int j = 0; j < 2; ++j) {
+                  float& y = x[mt][nt][2 * i + j];
+                  const float e = ex2(y - finite_or_zero(m[nt][j]));
+                  l[nt][j] += e;
+                  y = e * vs;
+                  top_w[nt][j] = fmaxf(top_w[nt][j], y);
+                }
+            }
+          bool over = false;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) over |= top_w[nt][j] * winv[nt][j] > kWeightTop;
+          if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                float t = top_w[nt][j];
+                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
+                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
+                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
+                if (!(t * winv[nt][j] > kWeightTop)) continue;
+                // t into [2^10, 2^11); what was summed follows
+                const uint32_t to = min(kWeightMost, 127 + 10 + 127 - (__float_as_uint(t) >> 23));
+                const int down = static_cast<int>(to - (__float_as_uint(winv[nt][j]) >> 23));
+                const float f = down > -127 ? __uint_as_float(static_cast<uint32_t>(127 + down) << 23) : 0.f;
+                winv[nt][j] = __uint_as_float(to << 23);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                  o[dt][nt][j] *= f;
+                  o[dt][nt][2 + j] *= f;
+                }
+              }
           }
-          vinv = 1.f / vref;
         }
         // ---- O^T += V^T P^T
 #pragma unroll
@@ -594,14 +637,15 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              float e0 = ex2(x[mt][nt][2 * i] - finite_or_zero(m[nt][0]));
-              float e1 = ex2(x[mt][nt][2 * i + 1] - finite_or_zero(m[nt][1]));
-              l[nt][0] += e0;
-              l[nt][1] += e1;
+              float e0, e1;
               if constexpr (C::kFp8) {
-                const float vs = scales[C::kKeys + mt * 16 + i * 8 + row] * vinv;
-                e0 *= vs;
-                e1 *= vs;
+                e0 = x[mt][nt][2 * i] * winv[nt][0];
+                e1 = x[mt][nt][2 * i + 1] * winv[nt][1];
+              } else {
+                e0 = ex2(x[mt][nt][2 * i] - finite_or_zero(m[nt][0]));
+                e1 = ex2(x[mt][nt][2 * i + 1] - finite_or_zero(m[nt][1]));
+                l[nt][0] += e0;
+                l[nt][1] += e1;
               }
               const uint32_t high = pack16<C::kBf16>(e0, e1);
               pb[nt][i] = transpose8(high);
@@ -673,7 +717,7 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) sum += sm_l[w * NT * 8 + i] * ex2(sm_m[w * NT * 8 + i] - ref);
         float f = ex2(m[nt][j] - ref);
-        if constexpr (C::kFp8) f *= vref;
+        if constexpr (C::kFp8) f *= __uint_as_float((254u << 23) - __float_as_uint(winv[nt][j]));
         m[nt][j] = top;
         l[nt][j] = sum;
 #pragma unroll

@@ -74,6 +74,84 @@ def check(q, cache, table, lengths):
         assert (np.abs(lse64[b] - ref["lse"]) <= bound["lse"]).all(), (b, n)
 
 
+@pytest.mark.parametrize("kv, half", [("bf16", "bf16"), ("fp16", "fp16"), ("e4m3", "bf16"), ("e4m3", "fp16")])
+@pytest.mark.parametrize("D, H, G", [(128, 2, 1), (64, 2, 8), (128, 1, 16), (256, 2, 4), (32, 1, 20)])
+def test_what_is_rounded(kv, half, D, H, G):
+    lengths = [1, 2, 3, 5, 6, 17, 64, 129, 300]
+    cache, table, n, _, _ = filled(lengths, H, 16, D, kv, half=DTYPES[half], seed=D + G)
+    check(rows((len(lengths), H * G, D), DTYPES[half], 5, 0.5), cache, table, n)
+
+
+def one_far_key(n, at, D, log2_weight, half, seed):
+    """q rows and keys of small scores, but for key ``at`` of each sequence,
+    whose weight is about 2^log2_weight of the others'."""
+    g = torch.Generator().manual_seed(seed)
+    base = torch.randn((D,), generator=g).sign()
+    q = (base + 0.05 * torch.randn((len(at), 4, D), generator=g)).to(half)
+    k = 0.05 * torch.randn((len(at), n, 1, D), generator=g)
+    for b, i in enumerate(at):
+        k[b, i] = base * (log2_weight * math.log(2.0) / math.sqrt(D))
+    return q.cuda(), k.to(half).cuda(), g
+
+
+@pytest.mark.parametrize("half", ["bf16", "fp16"])
+@pytest.mark.parametrize("ratio", [1e2, 1e4, 1e6, 1e7, 2.0**26, 1e12, 1e20])
+def test_a_large_value_row_of_no_weight_costs_the_others_nothing(ratio, half):
+    """e4m3: one V row ``ratio`` times the others, its key's weight 2^-100."""
+    from repercep_runtime_b200 import paged
+
+    if half == "fp16" and ratio > 1e6:
+        pytest.skip("fp16 holds no such values")
+    n, at, D = 520, [0, 100, 263, 519], 128
+    q, k, g = one_far_key(n, at, D, -100.0, DTYPES[half], 3)
+    small = 1e-2 if half == "fp16" else 1.0
+    v = small * torch.randn((len(at), n, 1, D), generator=g)
+    for b, i in enumerate(at):
+        v[b, i] = (small * ratio * torch.randn((1, D), generator=g)).clamp(-6e4, 6e4) if half == "fp16" else (
+            ratio * torch.randn((1, D), generator=g))
+    cache, table, lengths, _, _ = filled([n] * len(at), 1, 16, D, "e4m3", half=DTYPES[half], seed=1)
+    starts = torch.arange(0, len(at) * n + 1, n, dtype=torch.int32, device="cuda")
+    paged.append(cache, k.view(-1, 1, D), v.to(DTYPES[half]).cuda().view(-1, 1, D), table, torch.zeros_like(lengths), starts=starts)
+    check(q, cache, table, lengths)
+
+
+@pytest.mark.parametrize("kv, half", [("bf16", "bf16"), ("e4m3", "bf16"), ("e4m3", "fp16")])
+@pytest.mark.parametrize("log2_weight", [4.0, 13.0, 20.0, 26.0, 30.0])
+def test_small_weights_beside_a_dominant_key(kv, half, log2_weight):
+    """A key 2^log2_weight times as heavy as each of the others, whose V row has
+    nothing in most dimensions: the others make those."""
+    from repercep_runtime_b200 import paged
+
+    n, at, D = 1500, [0, 700, 1499], 64
+    q, k, g = one_far_key(n, at, D, log2_weight, DTYPES[half], 4)
+    v = 2e4 * (1.0 + 0.3 * torch.randn((len(at), n, 1, D), generator=g))
+    for b, i in enumerate(at):
+        v[b, i] = 0.0
+        v[b, i, 0, :4] = 1.0
+    cache, table, lengths, _, _ = filled([n] * len(at), 1, 32, D, kv, half=DTYPES[half], seed=2)
+    starts = torch.arange(0, len(at) * n + 1, n, dtype=torch.int32, device="cuda")
+    paged.append(cache, k.view(-1, 1, D), v.to(DTYPES[half]).cuda().view(-1, 1, D), table, torch.zeros_like(lengths), starts=starts)
+    check(q, cache, table, lengths)
+
+
+@pytest.mark.parametrize("kv", ["fp16", "e4m3"])
+def test_scores_that_keep_rising(kv):
+    """Ascending scores move the reference of the weights again and again; the
+    V rows fall as they rise."""
+    from repercep_runtime_b200 import paged
+
+    n, D, half = 900, 64, torch.float16 if kv == "fp16" else torch.bfloat16
+    g = torch.Generator().manual_seed(6)
+    base = torch.randn((D,), generator=g).sign()
+    q = base.repeat(1, 4, 1).to(half).cuda()
+    k = (base * torch.linspace(0.0, 80.0, n).view(1, n, 1, 1) / math.sqrt(D)).to(half).cuda()
+    v = (torch.randn((1, n, 1, D), generator=g) * torch.exp2(-torch.linspace(-8.0, 8.0, n)).view(1, n, 1, 1)).to(half).cuda()
+    cache, table, lengths, _, _ = filled([n], 1, 16, D, kv, half=half, seed=3)
+    starts = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    paged.append(cache, k.view(-1, 1, D), v.view(-1, 1, D), table, torch.zeros_like(lengths), starts=starts)
+    check(q, cache, table, lengths)
+
+
 @pytest.mark.parametrize("D", [32, 64, 128, 256])
 @pytest.mark.parametrize("layout", ["bhsd", "bshd"])
 def test_zero_and_tiny_fp16_rows_in_an_e4m3_cache(D, layout):
