@@ -367,7 +367,8 @@ int rp_paged_decode_workspace_bytes(const rp_paged_kv* kv, int B, int Hq, int ta
  *        execution
  * A sequence of length 0 gives out = 0 and lse = -inf.  sm_scale <= 0 selects
  * 1/sqrt(head_dim).  Scores, sums and accumulators are fp32; softmax weights
- * enter their product with V as a 16-bit value and a 16-bit remainder.  With an
+ * enter their product with V as a 16-bit value and a 16-bit remainder (fp16: to
+ * 2^-36 of the query head's largest).  With an
  * e4m3 cache a weight times its row's V scale is rounded once, to fp16 (by
  * 2^-11 of itself, or 2^-35 of the query head's largest such product), and the
  * queries are rounded to fp16 after a power of two of their row's maximum

@@ -34,9 +34,10 @@
 //    16-bit V a softmax weight is split into a 16-bit value and the 16-bit
 //    remainder, two products each, which cost 1 % of the time; rounded once it
 //    added as much error as the output's own rounding (2.2e-3 against 1.7e-3 in
-//    all).  With an e4m3 cache it is rounded once, with its V scale, to fp16:
-//    relative 2^-11, and absolutely 2^-35 of the column's largest such product
-//    (two parts there cost 2 to 10 %: 233 us for the batch below, 73 for 16 heads).
+//    all); an fp16 pair holds 2^-36 of the row's largest weight.  With an e4m3
+//    cache it is rounded once, with its V scale, to fp16: relative 2^-11, and
+//    absolutely 2^-35 of the column's largest such product (two parts there cost
+//    2 to 10 %: 233 us for the batch below, 73 for 16 heads a KV head).
 // Measured, main kernel: two sequences of 115k tokens, 32/8 heads, fp16 144 us
 // (6.9 TB/s); 64 sequences of 512 to 520, 32/32 heads, bf16, with scores kept for
 // the weights 84 us (6.5 TB/s); 128 of 1 to 8191, 32/8 heads, e4m3, with scores
@@ -76,8 +77,10 @@ struct Cfg {
   static constexpr int kFrags = D / 16 * NT;  // accumulator fragments (float4 a lane)
   // The reference m of a row's weights 2^(s - m) (log2 units): a new one lies kBelow
   // under the maximum, and stays until a score exceeds it by kAbove.  e4m3: weights
-  // are at most 1, so that a product with any V scale is finite.
-  static constexpr float kBelow = kFp8 ? -8.f : 0.f, kAbove = kBelow + 8.f;
+  // are at most 1, so that a product with any V scale is finite.  fp16: the largest
+  // lie in [2^11, 2^15], so that small ones keep clear of the format's lower end.
+  static constexpr float kBelow = kFp8 ? -8.f : kBf16 ? 0.f : 11.f;
+  static constexpr float kAbove = kFp8 ? 0.f : kBf16 ? 8.f : 15.f;
   // keys of a warp's step: 16 where that makes 8 KB (a stage holds a warp's accumulators at times)
   static constexpr int kKeys = 32 * kRow >= 8192 && 32 * kRow >= kFrags * 512 ? 16 : 32;
   static constexpr int kTile = kKeys * kWarps;

@@ -115,7 +115,7 @@ def test_a_large_value_row_of_no_weight_costs_the_others_nothing(ratio, half):
     check(q, cache, table, lengths)
 
 
-@pytest.mark.parametrize("kv, half", [("bf16", "bf16"), ("e4m3", "bf16"), ("e4m3", "fp16")])
+@pytest.mark.parametrize("kv, half", [("bf16", "bf16"), ("fp16", "fp16"), ("e4m3", "bf16"), ("e4m3", "fp16")])
 @pytest.mark.parametrize("log2_weight", [4.0, 13.0, 20.0, 26.0, 30.0])
 def test_small_weights_beside_a_dominant_key(kv, half, log2_weight):
     """A key 2^log2_weight times as heavy as each of the others, whose V row has
