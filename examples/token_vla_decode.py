@@ -122,6 +122,7 @@ def plan(
     own = -(-steps // c.page)  # pages of a candidate's own
     prompt_pages = -(-P // c.page)
     x = model.embed[prompt]
+    upto = torch.arange(1, P + 1, dtype=torch.int32, device="cuda")  # tokens of the prompt up to each
     kept = None
     caches, tables = [], []
     for layer in range(c.layers):
@@ -137,10 +138,10 @@ def plan(
         rows = [t.transpose(0, 1).unsqueeze(0) for t in (q, k.repeat_interleave(group, 1), v.repeat_interleave(group, 1))]
         attended = ops.fp8_attention(*(t.contiguous() for t in rows), causal=True, scale_mode=ops.SCALE_PER_BLOCK128)
         if stay < P:
-            # weights of the last tokens' queries: one call each, all over the whole prompt
+            # weights of the last tokens' queries: one call each, over the prompt up to its own token
             weights = torch.zeros((1, c.kv_heads, table.shape[1] * c.page), device="cuda")
-            for t in range(P - observe, P):
-                paged.decode(q[t : t + 1], cache, table, lengths, weights=weights)
+            for t in range(max(0, P - observe), P):
+                paged.decode(q[t : t + 1], cache, table, upto[t : t + 1], weights=weights)
             new_rows = pages.take(stay // c.page)
             cut = paged.evict(cache, table, lengths, weights, table_of([new_rows]), budget=stay, recent=observe)
             pages.give(table_rows)
