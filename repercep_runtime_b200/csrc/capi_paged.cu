@@ -10,6 +10,8 @@ namespace {
 
 using rp::set_last_error;
 
+constexpr float kLog2e = 1.4426950408889634f;
+
 bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 int launched(cudaError_t e, const char* what) {
@@ -161,7 +163,7 @@ int rp_paged_decode(const rp_paged_kv* kv, const void* q, const int64_t* q_strid
   if (rp::pool_unit(a.kv) == 0)
     return set_last_error(RP_ERR_UNSUPPORTED, "the pool's strides address more than 2^32 units of their common power of two");
   if (Hq > 65535) return set_last_error(RP_ERR_UNSUPPORTED, "more than 65535 query heads");
-  if (!std::isfinite(sm_scale)) return set_last_error(RP_ERR_INVALID, "sm_scale is not finite");
+  if (!std::isfinite(sm_scale * kLog2e)) return set_last_error(RP_ERR_INVALID, "sm_scale is not finite in log2 units");
   if (B == 0) return RP_OK;
   if (!q || !q_strides || !out || !out_strides) return set_last_error(RP_ERR_INVALID, "q or out is null");
   if (!aligned(q, 16) || q_strides[0] % 8 != 0 || q_strides[1] % 8 != 0)
@@ -176,7 +178,7 @@ int rp_paged_decode(const rp_paged_kv* kv, const void* q, const int64_t* q_strid
   a.q_f16 = q_dtype == RP_DTYPE_F16;
   a.Hq = Hq;
   const float scale = sm_scale > 0.f ? sm_scale : 1.f / std::sqrt(static_cast<float>(a.kv.D));
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.scale_log2 = scale * kLog2e;
   a.out = static_cast<uint16_t*>(out);
   a.o_seq = out_strides[0];
   a.o_head = out_strides[1];

@@ -29,7 +29,7 @@ raises).
 from __future__ import annotations
 
 import functools
-from ctypes import byref, c_int64
+from ctypes import byref, c_float, c_int64
 from dataclasses import dataclass, field
 from typing import NamedTuple
 
@@ -271,8 +271,10 @@ def decode(
     q0, q1, q2 = q.stride()
     if q2 != 1:
         raise ValueError("q must have a unit-stride head dim")
-    if scale is not None and not 0.0 < scale < float("inf"):
-        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if scale is not None:
+        given, scale = scale, c_float(scale).value  # as the library takes it, where 0 means 1 / sqrt(D)
+        if not 0.0 < scale < float("inf"):
+            raise ValueError(f"scale must be positive and finite in fp32, got {given}")
     if out is None:
         out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
     elif out.shape != shape or out.dtype != dtype or out.device != device or out.stride(2) != 1:
@@ -286,7 +288,7 @@ def decode(
     ws = torch.empty(need, dtype=torch.uint8, device=device)
     _lib.launch(
         device.index, "rp_paged_decode", cache._struct(), q.data_ptr(), _I64x2(q0, q1), _HALF[dtype], B, Hq,
-        page_table.data_ptr(), row, pages, lengths.data_ptr(), 0.0 if scale is None else float(scale),
+        page_table.data_ptr(), row, pages, lengths.data_ptr(), 0.0 if scale is None else scale,
         out.data_ptr(), _I64x2(o0, o1), None if lse is None else lse.data_ptr(), w, w_strides, w_cols,
         ws.data_ptr(), need,
     )  # fmt: skip
