@@ -51,7 +51,7 @@ int pool_of(const rp_paged_kv* kv, bool data, rp::PagedPool* p) {
 int check_capacity(const char* what, int pages, int64_t stride, int page_size) {
   if (pages < 0 || (pages > 0 && stride < pages))
     return set_last_error(RP_ERR_INVALID, "%s: %d pages a row, %lld apart", what, pages, (long long)stride);
-  if (static_cast<int64_t>(pages) * page_size > 0x7FFFFFFF - 4096)
+  if (static_cast<int64_t>(pages) * page_size > rp::kMaxPositions)
     return set_last_error(RP_ERR_UNSUPPORTED, "%s: a sequence of more than 2^31 positions", what);
   return RP_OK;
 }

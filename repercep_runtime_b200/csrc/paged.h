@@ -13,6 +13,11 @@ constexpr int kStatusBadPage = 0x201;    // a page id outside the pool
 constexpr int kStatusBadLength = 0x202;  // a length below 0 or past the page table, bad starts
 constexpr int kStatusBadToken = 0x203;   // a token id past the vocabulary
 
+// Positions that a page table addresses, at most: loops over them step past the
+// end by a grid's stride (4096 a CTA cluster, 1024 positions a CTA of the weights'
+// launch), which has to fit an int.
+constexpr int kMaxPositions = 0x7FFFFFFF - (1 << 23);
+
 // Value types of a cache (rp_kv_dtype).
 constexpr int kKvBf16 = 0, kKvF16 = 1, kKvE4m3 = 2;
 

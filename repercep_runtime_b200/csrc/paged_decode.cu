@@ -1057,7 +1057,9 @@ cudaError_t launch_paged_decode(const PagedDecodeArgs& a, cudaStream_t st) {
   // enough CTAs for the SMs, at most one per 1024 positions
   const int rows = a.kv.heads * a.t.B, most = (cap + 1023) / 1024;
   const int want = (16 * sm_count(current_device()) + rows - 1) / rows;
-  return launch_after(decode_weights_kernel, dim3(want < most ? want : most, a.kv.heads, a.t.B), 256, 0, st, p);
+  const int ctas = want < most ? want : most;
+  if (static_cast<int64_t>(ctas) * 1024 > 0x7FFFFFFF - kMaxPositions) return cudaErrorInvalidValue;
+  return launch_after(decode_weights_kernel, dim3(ctas, a.kv.heads, a.t.B), 256, 0, st, p);
 }
 
 }  // namespace rp

@@ -2,10 +2,24 @@
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
-from test_paged_cpu import decode, lib  # noqa: F401
+from test_paged_cpu import DUMMY, append, decode, evict, kv, lib  # noqa: F401
 
 
 @pytest.mark.parametrize("scale", [3e38, -3e38, float("inf")])
 def test_a_scale_that_log2_units_do_not_hold_is_refused(lib, scale):  # noqa: F811
     assert decode(lib, scale=scale) == -1 and b"finite" in lib.rp_last_error()
+
+
+def test_tables_whose_loops_would_pass_2_31_are_refused(lib):  # noqa: F811
+    """A loop over positions steps past its end by up to 2^23: an int that wraps
+    there would index memory before the weights."""
+    pages = (2**31 - 8192) // 16
+    n = ctypes.c_size_t()
+    assert lib.rp_paged_decode_workspace_bytes(kv(), 1, 2, pages, 1, ctypes.byref(n)) == -2
+    assert b"2^31" in lib.rp_last_error()
+    for call in (append, decode, evict):
+        assert call(lib, pages=pages, stride=pages, weights=DUMMY, cols=1 << 31) == -2 and b"2^31" in lib.rp_last_error()
+    assert lib.rp_paged_decode_workspace_bytes(kv(), 1, 2, (2**31 - 2**24) // 16, 1, ctypes.byref(n)) == 0
