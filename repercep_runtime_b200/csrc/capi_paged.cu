@@ -163,6 +163,8 @@ int rp_paged_decode(const rp_paged_kv* kv, const void* q, const int64_t* q_strid
   if (rp::pool_unit(a.kv) == 0)
     return set_last_error(RP_ERR_UNSUPPORTED, "the pool's strides address more than 2^32 units of their common power of two");
   if (Hq > 65535) return set_last_error(RP_ERR_UNSUPPORTED, "more than 65535 query heads");
+  if (static_cast<int64_t>(B) * Hq > 0x7FFFFFFF)
+    return set_last_error(RP_ERR_UNSUPPORTED, "more than 2^31 query rows");
   if (!std::isfinite(sm_scale * kLog2e)) return set_last_error(RP_ERR_INVALID, "sm_scale is not finite in log2 units");
   if (B == 0) return RP_OK;
   if (!q || !q_strides || !out || !out_strides) return set_last_error(RP_ERR_INVALID, "q or out is null");

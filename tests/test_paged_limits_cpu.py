@@ -23,3 +23,8 @@ def test_tables_whose_loops_would_pass_2_31_are_refused(lib):  # noqa: F811
     for call in (append, decode, evict):
         assert call(lib, pages=pages, stride=pages, weights=DUMMY, cols=1 << 31) == -2 and b"2^31" in lib.rp_last_error()
     assert lib.rp_paged_decode_workspace_bytes(kv(), 1, 2, (2**31 - 2**24) // 16, 1, ctypes.byref(n)) == 0
+
+
+def test_more_query_rows_than_an_int_holds_are_refused(lib):  # noqa: F811
+    """B * query heads numbers the items that CTAs leave to each other."""
+    assert decode(lib, B=65535, Hq=40000) == -2 and b"2^31" in lib.rp_last_error()
