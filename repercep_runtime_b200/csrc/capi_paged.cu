@@ -30,6 +30,9 @@ int pool_of(const rp_paged_kv* kv, bool data, rp::PagedPool* p) {
     return set_last_error(RP_ERR_INVALID, "num_pages, heads and page_size must be positive");
   if (kv->heads > 65535) return set_last_error(RP_ERR_UNSUPPORTED, "more than 65535 KV heads");
   const bool e4m3 = kv->dtype == RP_KV_E4M3;
+  // a stride that no offset uses is any number
+  const int64_t strides[3] = {kv->num_pages > 1 ? kv->strides[0] : 0, kv->heads > 1 ? kv->strides[1] : 0,
+                              kv->page_size > 1 ? kv->strides[2] : 0};
   if (data) {
     if (!kv->k || !kv->v) return set_last_error(RP_ERR_INVALID, "k or v is null");
     if (e4m3 && (!kv->k_scales || !kv->v_scales))
@@ -38,12 +41,12 @@ int pool_of(const rp_paged_kv* kv, bool data, rp::PagedPool* p) {
     if (!aligned(kv->k, 16) || !aligned(kv->v, 16))
       return set_last_error(RP_ERR_ALIGN, "k and v must be 16-byte aligned");
     for (int i = 0; i < 3; ++i)
-      if (kv->strides[i] % unit != 0 || kv->strides[i] < 0)
+      if (strides[i] % unit != 0 || strides[i] < 0)
         return set_last_error(RP_ERR_ALIGN, "cache stride %d must be a non-negative multiple of 16 bytes", i);
   }
   *p = rp::PagedPool{static_cast<uint8_t*>(kv->k), static_cast<uint8_t*>(kv->v),
                      e4m3 ? kv->k_scales : nullptr, e4m3 ? kv->v_scales : nullptr,
-                     kv->strides[0], kv->strides[1], kv->strides[2],
+                     strides[0], strides[1], strides[2],
                      kv->dtype, kv->num_pages, kv->heads, kv->page_size, kv->head_dim};
   return RP_OK;
 }
@@ -111,13 +114,12 @@ int rp_paged_append(const rp_paged_kv* kv, const void* k_new, const void* v_new,
     if (!k_new || !v_new || !new_strides) return set_last_error(RP_ERR_INVALID, "new rows are null");
     if (!aligned(k_new, 16) || !aligned(v_new, 16))
       return set_last_error(RP_ERR_ALIGN, "new rows must be 16-byte aligned");
-    for (int i = 0; i < 4; ++i)
-      if (new_strides[i] % 8 != 0)
-        return set_last_error(RP_ERR_ALIGN, "new row strides must be multiples of 8 elements");
-    a.k_tok = new_strides[0];
-    a.k_head = new_strides[1];
-    a.v_tok = new_strides[2];
-    a.v_head = new_strides[3];
+    a.k_tok = tokens > 1 ? new_strides[0] : 0;
+    a.k_head = a.kv.heads > 1 ? new_strides[1] : 0;
+    a.v_tok = tokens > 1 ? new_strides[2] : 0;
+    a.v_head = a.kv.heads > 1 ? new_strides[3] : 0;
+    for (const int64_t s : {a.k_tok, a.k_head, a.v_tok, a.v_head})
+      if (s % 8 != 0) return set_last_error(RP_ERR_ALIGN, "new row strides must be multiples of 8 elements");
   }
   if ((rc = rp::device_ready(&a.status)) != RP_OK) return rc;
   a.k_new = static_cast<const uint16_t*>(k_new);
@@ -168,15 +170,15 @@ int rp_paged_decode(const rp_paged_kv* kv, const void* q, const int64_t* q_strid
   if (!std::isfinite(sm_scale * kLog2e)) return set_last_error(RP_ERR_INVALID, "sm_scale is not finite in log2 units");
   if (B == 0) return RP_OK;
   if (!q || !q_strides || !out || !out_strides) return set_last_error(RP_ERR_INVALID, "q or out is null");
-  if (!aligned(q, 16) || q_strides[0] % 8 != 0 || q_strides[1] % 8 != 0)
+  a.q_seq = B > 1 ? q_strides[0] : 0;
+  a.q_head = Hq > 1 ? q_strides[1] : 0;
+  if (!aligned(q, 16) || a.q_seq % 8 != 0 || a.q_head % 8 != 0)
     return set_last_error(RP_ERR_ALIGN, "q and its strides must be 16-byte multiples");
   const size_t need = rp::paged_decode_workspace(a.kv, B, Hq, table_pages, weights != nullptr);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return set_last_error(RP_ERR_WORKSPACE, "a 16-byte aligned workspace of %zu bytes required", need);
   if ((rc = rp::device_ready(&a.status)) != RP_OK) return rc;
   a.q = static_cast<const uint16_t*>(q);
-  a.q_seq = q_strides[0];
-  a.q_head = q_strides[1];
   a.q_f16 = q_dtype == RP_DTYPE_F16;
   a.Hq = Hq;
   const float scale = sm_scale > 0.f ? sm_scale : 1.f / std::sqrt(static_cast<float>(a.kv.D));

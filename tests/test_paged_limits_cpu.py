@@ -28,3 +28,10 @@ def test_tables_whose_loops_would_pass_2_31_are_refused(lib):  # noqa: F811
 def test_more_query_rows_than_an_int_holds_are_refused(lib):  # noqa: F811
     """B * query heads numbers the items that CTAs leave to each other."""
     assert decode(lib, B=65535, Hq=40000) == -2 and b"2^31" in lib.rp_last_error()
+
+
+def test_a_stride_that_no_offset_uses_is_any_number(lib):  # noqa: F811
+    """One sequence, one page, one head: the call gets as far as the workspace."""
+    for pool, changes in [(None, dict(B=1, q_strides=(513, 128))), (kv(num_pages=1, strides=(4097, 2048, 128)), {}),
+                          (kv(heads=1, strides=(2048, 3, 128)), {}), (kv(page_size=1, strides=(256, 128, 5)), {})]:
+        assert decode(lib, pool, ws=None, **changes) == -6, lib.rp_last_error()
