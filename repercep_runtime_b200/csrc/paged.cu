@@ -182,13 +182,13 @@ cudaError_t append_u(const AppendArgs& a, cudaStream_t st) {
   return cudaGetLastError();
 }
 
-// Two rows a thread once the GPU is full all the same (148 SMs of 2048 threads):
+// Two rows a thread once the GPU is full all the same (2048 threads an SM):
 // the 48 prompts take 115 us with two, 132 with one, 145 with four; 49k rows of
 // e4m3, which fill two thirds of it, 12.2 us with two and 11.2 with one.
 template <int D>
 cudaError_t append_d(const AppendArgs& a, cudaStream_t st) {
   const int64_t threads = static_cast<int64_t>(a.tokens) * a.kv.heads * (D / 8 / (a.kv.dtype == kKvE4m3 ? 2 : 1));
-  return threads >= 2LL * 148 * 2048 ? append_u<D, 2>(a, st) : append_u<D, 1>(a, st);
+  return threads >= 2LL * 2048 * sm_count(current_device()) ? append_u<D, 2>(a, st) : append_u<D, 1>(a, st);
 }
 
 // Weights order: a key is larger when the weight is; -0 equals 0 and any NaN
@@ -546,7 +546,7 @@ cudaError_t launch_paged_evict(const EvictArgs& a, cudaStream_t st) {
   int parts = 1;
   // a larger cluster while the slices are long and the GPU holds all CTAs at once (three an SM)
   while (parts < most && cap > static_cast<int64_t>(parts) * kSliceAim &&
-         static_cast<int64_t>(a.kv.heads) * a.t.B * parts * 2 <= 148 * 3)
+         static_cast<int64_t>(a.kv.heads) * a.t.B * parts * 2 <= 3 * sm_count(dev))
     parts *= 2;
   const int64_t per = (cap + parts - 1) / parts;
   const bool held = per <= kSliceHeld;

@@ -2,6 +2,7 @@
 // decode, evict) and of token scoring.
 #pragma once
 
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
 #include <cuda_runtime.h>
@@ -138,6 +139,14 @@ constexpr int kMaxDevices = 64;
 inline int current_device() {
   int dev = 0;
   return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < kMaxDevices ? dev : 0;
+}
+// SMs of a device (148 on a whole B200), 0 if it cannot be asked.
+inline int sm_count(int dev) {
+  static std::atomic<int> known[kMaxDevices];
+  int n = known[dev].load(std::memory_order_relaxed);
+  if (n == 0 && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess)
+    known[dev].store(n, std::memory_order_relaxed);
+  return n;
 }
 
 #ifdef __CUDACC__

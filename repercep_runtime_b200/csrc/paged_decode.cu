@@ -939,14 +939,6 @@ __global__ void __launch_bounds__(256) decode_weights_kernel(const Params p) {
   }
 }
 
-int sm_count(int dev) {
-  static std::atomic<int> known[kMaxDevices];
-  int n = known[dev].load(std::memory_order_relaxed);
-  if (n == 0 && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess)
-    known[dev].store(n, std::memory_order_relaxed);
-  return n;
-}
-
 // Column blocks of 8 query heads that a group of G heads is given: two at most
 // (a group of more than 16 heads takes several passes over its keys).
 int column_blocks(int G) { return G > 8 ? 2 : 1; }

@@ -45,7 +45,6 @@ constexpr int kU = 4;                // 16-byte vectors of a thread's batch
 constexpr int kStages = 3;           // batches of a thread in shared memory
 constexpr int kRing = kStages * kU * kT * 16;  // bytes: 24 KB, five CTAs an SM
 constexpr int kResident = 5;
-constexpr int kSms = 148;
 constexpr int kSegments = 16;        // segments of a thread, at most
 constexpr int kCandidates = 512;     // values kept for the selection
 constexpr int kLook = 12;            // values of a thread in flight when segments are read again
@@ -502,16 +501,18 @@ template <int DT>
 cudaError_t launch(const ScoreArgs& a, cudaStream_t st) {
   // CTAs of a row: while the GPU holds all of them at once and each has two vectors a thread.
   constexpr int kVec = Type<DT>::kVec;
+  const int sms = sm_count(current_device());
+  if (sms <= 0) return cudaErrorInvalidDevice;
   const int64_t vectors = static_cast<int64_t>(a.vocab) / kVec + 2;
   int parts = 1;
-  while (parts < kMaxCluster && static_cast<int64_t>(a.rows) * parts * 2 <= kSms * kResident &&
+  while (parts < kMaxCluster && static_cast<int64_t>(a.rows) * parts * 2 <= sms * kResident &&
          vectors / (parts * 2) >= 2 * kT)
     parts *= 2;
   const int64_t batches = (vectors / parts + 1 + kU * kT - 1) / (kU * kT);  // of a thread
   const int per_segment = static_cast<int>((batches + kSegments - 1) / kSegments);
   const int64_t segments = (batches + per_segment - 1) / per_segment;
   const size_t smem = kRing + (a.top > 0 ? kCandidates * 8 + static_cast<size_t>(segments) * kT * 4 : 0);
-  const int rows = a.rows < kSms * kResident ? a.rows : kSms * kResident;  // at once
+  const int rows = a.rows < sms * kResident ? a.rows : sms * kResident;  // at once
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(rows) * parts);
   cfg.blockDim = dim3(kT);
