@@ -122,8 +122,10 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 // Cached rows leave L2 first and scores last: the rows are read once, while a
-// later launch reads the scores (e4m3 batch with weights: 225 us in all, 230
-// without the second).
+// later launch reads the scores (e4m3 batch with weights: 228 us in all, 234
+// without the second).  That launch gives their lines back: left as they were,
+// they kept part of L2 from the kernels that came after (80 MB summed again and
+// again took 20.5 us a pass instead of 16.4, with no end).
 __device__ __forceinline__ uint64_t evict_first() {
   uint64_t policy;
   asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
@@ -136,6 +138,19 @@ __device__ __forceinline__ uint64_t evict_last() {
 }
 __device__ __forceinline__ void store_kept(float* dst, float x, uint64_t policy) {
   asm volatile("st.global.L2::cache_hint.f32 [%0], %1, %2;" ::"l"(dst), "f"(x), "l"(policy) : "memory");
+}
+__device__ __forceinline__ float4 load_once(const float* src, uint64_t policy) {
+  float4 x;
+  asm volatile("ld.global.L1::no_allocate.L2::cache_hint.v4.f32 {%0, %1, %2, %3}, [%4], %5;"
+               : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+               : "l"(src), "l"(policy)
+               : "memory");
+  return x;
+}
+// The 128-byte line of `at` leaves L2 when its turn comes.
+__device__ __forceinline__ void give_back_line(const float* at) {
+  asm volatile("applypriority.global.L2::evict_normal [%0], 128;" ::"l"(reinterpret_cast<uint64_t>(at) & ~127ull)
+               : "memory");
 }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool read, uint64_t policy) {
   asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src),
@@ -906,6 +921,7 @@ __global__ void __launch_bounds__(256) decode_weights_kernel(const Params p) {
   const float* lse2 = p.lse2 + row;
   float* dst = p.a.weights.w + b * p.a.weights.s_seq + h * p.a.weights.s_head;
   const bool whole = (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
+  const uint64_t policy = evict_first();
   for (int j = (blockIdx.x * 256 + threadIdx.x) * 4; j < n; j += gridDim.x * 1024) {
     float w[4] = {0.f, 0.f, 0.f, 0.f}, old[4];
     const bool four = whole && j + 4 <= n;
@@ -923,7 +939,9 @@ __global__ void __launch_bounds__(256) decode_weights_kernel(const Params p) {
     for (int g = 0; g < p.G; ++g) {
       const float y = finite_or_zero(__ldcg(lse2 + g));
       // the rows of scores are whole 16-byte vectors; what lies past n is not used
-      const float4 x = __ldcs(reinterpret_cast<const float4*>(scores + static_cast<int64_t>(g) * p.score_pitch + j));
+      const float* src = scores + static_cast<int64_t>(g) * p.score_pitch + j;
+      const float4 x = load_once(src, policy);
+      if (threadIdx.x % 8 == 0) give_back_line(src);  // eight threads read a line
       w[0] += ex2(x.x - y);
       w[1] += ex2(x.y - y);
       w[2] += ex2(x.z - y);
