@@ -25,8 +25,8 @@ constexpr int kAppendThreads = 256;
 // V's amax share the words of one shuffle reduction over the row's D / 16 lanes,
 // and each lane then divides for one of the 2 U scales.  Reads 4 D bytes and
 // writes 2 D (or 4 D) a row, bound by HBM.  Measured: 48 prompts of 512 to 4099
-// tokens, 8 heads of 128, into an e4m3 cache 115 us, 6.2 TB/s; one token of 64
-// sequences 2.8 us.
+// tokens, 8 heads of 128, into an e4m3 cache 113 us, 6.3 TB/s (replayed in a
+// graph), into a bf16 one 147, 6.3 TB/s; one token of 64 sequences 2.4 us.
 template <int D, bool E4M3, bool F16, int U>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs a) {
   constexpr int kVecs = E4M3 ? 2 : 1;               // 16-byte vectors of a thread: it writes 16 bytes of K and of V
@@ -217,8 +217,9 @@ __device__ __forceinline__ float key_weight(uint32_t k) {
 // weights are equal: 57 us against 52 for two long sequences.)  Two passes more
 // count and place what is kept in order, so ties at the threshold go to the
 // lowest positions.  Reads each weight from HBM once; bound by the latency of
-// its few dependent passes, which the split over a cluster shortens.  Measured:
-// 16 rows of 70001 and 98303 weights 23 us, 128 rows of 1001 to 16385 19 us.
+// its few dependent passes, which the split over a cluster shortens.  Measured
+// (replayed in a graph, with the move of the 64 rows kept): 16 rows of 70001 and
+// 98303 weights 19 us, 128 rows of 1001 to 16385 18 us.
 constexpr int kSelThreads = 256;
 constexpr int kSelWarps = kSelThreads / 32;
 static_assert(kSelThreads >= 256, "a thread for every sum of 8 bins");
@@ -440,8 +441,8 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
 //
 // Kept rows to their new places: a warp takes 8 rows, their places found by 8
 // lanes, with K and V of all of them in flight before the first store.  Bound by
-// HBM: 4096 rows of 128 sequences and heads (bf16, D 128) 85 us, 6.1 TB/s read
-// and written.
+// HBM: 4096 rows of 128 sequences and heads (bf16, D 128) 85 us under the
+// profiler, 6.1 TB/s read and written; 100 us with the selection's launch.
 constexpr int kMoveRows = 8;
 constexpr int kMoveWarps = 8;
 
@@ -544,7 +545,9 @@ cudaError_t launch_paged_evict(const EvictArgs& a, cudaStream_t st) {
   }
   const int64_t cap = static_cast<int64_t>(a.t.pages) * a.kv.page_size;
   int parts = 1;
-  // a larger cluster while the slices are long and the GPU holds all CTAs at once (three an SM)
+  // a larger cluster while the slices are long and the GPU holds all CTAs at once: three an SM at
+  // slices of kSliceAim, fewer at longer ones, which then run in turns (96 rows of 98303 in
+  // clusters of four 80 us, of eight 63, of two 224: those slices do not fit the shared memory)
   while (parts < most && cap > static_cast<int64_t>(parts) * kSliceAim &&
          static_cast<int64_t>(a.kv.heads) * a.t.B * parts * 2 <= 3 * sm_count(dev))
     parts *= 2;

@@ -38,11 +38,11 @@
 //    cache it is rounded once, with its V scale, to fp16: relative 2^-11, and
 //    absolutely 2^-35 of the column's largest such product (two parts there cost
 //    2 to 10 %: 233 us for the batch below, 73 for 16 heads a KV head).
-// Measured, main kernel: two sequences of 115k tokens, 32/8 heads, fp16 144 us
-// (6.9 TB/s); 64 sequences of 512 to 520, 32/32 heads, bf16, with scores kept for
-// the weights 84 us (6.5 TB/s); 128 of 1 to 8191, 32/8 heads, e4m3, with scores
-// 196 us (5.9 TB/s, the scores' writes included).  The join takes 5 us, the
-// weights of that last batch 20 us (their traffic).
+// Measured (whole calls, replayed in a graph): two sequences of 115k tokens, 32/8
+// heads, fp16 155 us (6.4 TB/s); 64 sequences of 512 to 520, 32/32 heads, bf16 88
+// us (6.2 TB/s), with weights 92; 128 of 1 to 8191, 32/8 heads, e4m3, with weights
+// 224 us.  Under the profiler, caches flushed: main kernel, join and weights of
+// that batch 206, 8 and 21 us, the long case's main kernel 152 us (6.5 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>

@@ -22,9 +22,9 @@
 // that has another row to do starts it there before it selects the last one's
 // alternatives.
 // Few rows are split over a cluster of CTAs, joined through distributed shared
-// memory: one launch, no workspace.  Measured: 4095 x 100003 fp32, 20 alternatives
-// 303 us (5.4 TB/s; none: 259), 512 x 32000 bf16, 8 alternatives 14.5 us, one row of
-// 32000 over eight CTAs 9.4 us.
+// memory: one launch, no workspace.  Measured (replayed in a graph): 4095 x 100003
+// fp32, 20 alternatives 304 us (5.4 TB/s; none: 262), 512 x 32000 bf16, 8
+// alternatives 14.8 us, one row of 32000 over eight CTAs 9.3 us.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(kT, kResident) score_kernel(const ScoreArgs a,
         __syncthreads();
         const int hits = sh.hits, each = per_segment * kU * kVec;
         if (!strict && hits > kManyHits && have > kCandidates) return kCandidates + 1;
-        // (eight loads of a thread in flight: the row may have left L2)
+        // (kLook loads of a thread in flight: the row may have left L2)
         for (int i = t; i < hits * each; i += kLook * kT) {
           float y[kLook];
           int at[kLook];

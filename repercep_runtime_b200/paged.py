@@ -190,7 +190,8 @@ def append(
     fp16, behind the sequences' ``lengths``; returns the lengths after it.
 
     ``starts`` (sequences + 1,) int32 holds the first new token of each
-    sequence (tokens outside [starts[0], starts[-1]) are left out); without it
+    sequence (tokens outside [starts[0], starts[-1]) are left out, starts outside
+    the new tokens count as their ends); without it
     every sequence gets one token.  An e4m3 cache takes each row's scale and
     bytes from ``linear.quantize_rows``'s recipe.  ``weights`` are zeroed at
     the new positions.  Tokens past the page table are not counted; a sequence
