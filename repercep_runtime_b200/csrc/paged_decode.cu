@@ -121,8 +121,8 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// Cached rows leave L2 first and scores last: the rows are read once, while a
-// later launch reads the scores (e4m3 batch with weights: 228 us in all, 234
+// Cached rows leave L2 first and scores last: a row is read once (for every
+// sequence that names its page), while a later launch reads the scores (e4m3 batch with weights: 228 us in all, 234
 // without the second).  That launch gives their lines back: left as they were,
 // they kept part of L2 from the kernels that came after (80 MB summed again and
 // again took 20.5 us a pass instead of 16.4, with no end).
@@ -616,7 +616,7 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
                   const float e = ex2(y - finite_or_zero(m[nt][j]));
                   l[nt][j] += e;
                   y = e * vs;
-                  top_w[nt][j] = fmaxf(top_w[nt][j], y);
+                  top_w[nt][j] = fmaxf(top_w[nt][j], fabsf(y));
                 }
             }
           bool over = false;

@@ -64,8 +64,8 @@ def check(q, cache, table, lengths):
         p = np.exp(s - s.max(-1, keepdims=True))
         p /= p.sum(-1, keepdims=True)
         if e4m3:
-            safe = np.where(vs == 0.0, 1.0, vs)[:, None]
-            floor = 2.0**-35 * (p * vs[:, None]).max(-1, keepdims=True) / safe
+            size = np.abs(vs)[:, None]
+            floor = 2.0**-35 * (p * size).max(-1, keepdims=True) / np.where(size == 0.0, 1.0, size)
         else:
             floor = np.broadcast_to(2.0**-36 * p.max(-1, keepdims=True) if cache.dtype == torch.float16 else 0.0, p.shape)
         bound = op.decode_bound(q64[b], k, v, scale, u_out, u, floor.reshape(H * G, n))
@@ -132,6 +132,14 @@ def test_small_weights_beside_a_dominant_key(kv, half, log2_weight):
     starts = torch.arange(0, len(at) * n + 1, n, dtype=torch.int32, device="cuda")
     paged.append(cache, k.view(-1, 1, D), v.to(DTYPES[half]).cuda().view(-1, 1, D), table, torch.zeros_like(lengths), starts=starts)
     check(q, cache, table, lengths)
+
+
+def test_negative_scales_of_large_rows():
+    """A caller's own e4m3 cache may have multipliers of any sign."""
+    cache, table, n, _, _ = filled([300, 40], 2, 16, 64, "e4m3", seed=4)
+    cache.v_scales.copy_(torch.where(torch.arange(16, device="cuda") % 3 == 0, -1e6 * cache.v_scales, -cache.v_scales))
+    cache.k_scales.neg_()
+    check(rows((2, 4, 64), torch.bfloat16, 10), cache, table, n)
 
 
 @pytest.mark.parametrize("kv", ["fp16", "e4m3"])
