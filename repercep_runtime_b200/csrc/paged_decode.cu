@@ -64,7 +64,7 @@ constexpr int kMaxCtas = 592;  // CTAs of the main kernel, at most
 constexpr int kMinTiles = 2;    // tiles of a CTA's run, at least (but for the last)
 // e4m3: a weight times its row's V scale enters fp16 times a power of two of its
 // column's, which brings the largest such product to 2^10 or more, falls when one
-// exceeds 2^15, and is at most 2^110.
+// exceeds 2^15, rises as the weights fall with their reference, and is at most 2^110.
 constexpr float kWeightTop = 32768.f;
 constexpr uint32_t kWeightMost = 127 + 110;
 
@@ -77,8 +77,9 @@ struct Cfg {
   static constexpr int kFrags = D / 16 * NT;  // accumulator fragments (float4 a lane)
   // The reference m of a row's weights 2^(s - m) (log2 units): a new one lies kBelow
   // under the maximum, and stays until a score exceeds it by kAbove.  e4m3: weights
-  // are at most 1, so that a product with any V scale is finite.  fp16: the largest
-  // lie in [2^11, 2^15], so that small ones keep clear of the format's lower end.
+  // are at most 1, so that a product with any V scale is finite, and references are
+  // whole numbers.  fp16: the largest lie in [2^11, 2^15], so that small ones keep
+  // clear of the format's lower end.
   static constexpr float kBelow = kFp8 ? -8.f : kBf16 ? 0.f : 11.f;
   static constexpr float kAbove = kFp8 ? 0.f : kBf16 ? 8.f : 15.f;
   // keys of a warp's step: 16 where that makes 8 KB (a stage holds a warp's accumulators at times)
@@ -122,10 +123,11 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 // Cached rows leave L2 first and scores last: a row is read once (for every
-// sequence that names its page), while a later launch reads the scores (e4m3 batch with weights: 228 us in all, 234
-// without the second).  That launch gives their lines back: left as they were,
-// they kept part of L2 from the kernels that came after (80 MB summed again and
-// again took 20.5 us a pass instead of 16.4, with no end).
+// sequence that names its page), while a later launch reads the scores (e4m3 batch
+// with weights: 228 us in all, 234 without the second).  That launch gives their
+// lines back: left as they were, they kept part of L2 from the kernels that came
+// after (80 MB summed again and again took 20.5 us a pass instead of 16.4, with no
+// end).
 __device__ __forceinline__ uint64_t evict_first() {
   uint64_t policy;
   asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
@@ -587,10 +589,20 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
               t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
               t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
               t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
-              t = fmaxf(t - C::kBelow, m[nt][j]);
-              const float f = t == m[nt][j] ? 1.f : ex2(m[nt][j] - t);
-              m[nt][j] = t;
+              t -= C::kBelow;
+              if constexpr (C::kFp8) t = ceilf(t);  // whole, so that winv can follow
+              t = fmaxf(t, m[nt][j]);
+              float f = t == m[nt][j] ? 1.f : ex2(m[nt][j] - t);
               l[nt][j] *= f;
+              if constexpr (C::kFp8) {
+                // every product falls by 2^(t - m): winv takes that up, and the sums what it cannot
+                const uint32_t to = (__float_as_uint(winv[nt][j]) >> 23) +
+                                    (t == m[nt][j] ? 0 : static_cast<uint32_t>(fminf(t - m[nt][j], 400.f)));
+                const uint32_t left_over = to - min(to, kWeightMost);
+                winv[nt][j] = __uint_as_float(min(to, kWeightMost) << 23);
+                f = left_over < 127 ? __uint_as_float((127 - left_over) << 23) : 0.f;
+              }
+              m[nt][j] = t;
 #pragma unroll
               for (int dt = 0; dt < DT; ++dt) {
                 o[dt][nt][j] *= f;

@@ -134,6 +134,31 @@ def test_small_weights_beside_a_dominant_key(kv, half, log2_weight):
     check(q, cache, table, lengths)
 
 
+@pytest.mark.parametrize("kv, half", [("bf16", "bf16"), ("fp16", "fp16"), ("e4m3", "bf16"), ("e4m3", "fp16")])
+@pytest.mark.parametrize("ratio", [1e4, 1e8, 1e12, 1e25])
+@pytest.mark.parametrize("steps", [(60.0,), (20.0, 40.0, 100.0), (-30.0, 5.5, 31.25)])
+def test_large_value_rows_whose_weight_goes_later(kv, half, ratio, steps):
+    """Keys of large V rows lead until later keys outweigh them by 2^60 and more:
+    what those set must not hold the later ones down."""
+    from repercep_runtime_b200 import paged
+
+    if half == "fp16" and ratio > 1e8:
+        pytest.skip("fp16 holds no such values")
+    D, part, g = 64, 128 if len(steps) == 1 else 64, torch.Generator().manual_seed(8)
+    n = part * (len(steps) + 1)
+    base = torch.randn((D,), generator=g).sign()
+    q = (base + 0.05 * torch.randn((3, 4, D), generator=g)).to(DTYPES[half]).cuda()
+    level = torch.tensor([0.0, *steps]).repeat_interleave(part).view(1, n, 1, 1)  # log2 of the weights
+    k = base * level * math.log(2.0) / math.sqrt(D) + 0.05 * torch.randn((3, n, 1, D), generator=g)
+    top = 2e4 if half == "fp16" else ratio
+    v = torch.randn((3, n, 1, D), generator=g) * torch.logspace(math.log10(top), math.log10(top / ratio), len(steps) + 1).repeat_interleave(part).view(1, n, 1, 1)
+    cache, table, lengths, _, _ = filled([n] * 3, 1, 16, D, kv, half=DTYPES[half], seed=5)
+    starts = torch.arange(0, 3 * n + 1, n, dtype=torch.int32, device="cuda")
+    paged.append(cache, k.to(DTYPES[half]).cuda().view(-1, 1, D), v.clamp(-6e4, 6e4).to(DTYPES[half]).cuda().view(-1, 1, D) if half == "fp16"
+                 else v.to(DTYPES[half]).cuda().view(-1, 1, D), table, torch.zeros_like(lengths), starts=starts)
+    check(q, cache, table, lengths)
+
+
 def test_negative_scales_of_large_rows():
     """A caller's own e4m3 cache may have multipliers of any sign."""
     cache, table, n, _, _ = filled([300, 40], 2, 16, 64, "e4m3", seed=4)
